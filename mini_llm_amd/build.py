@@ -71,6 +71,9 @@ LIBRARIES: Dict[str, dict] = {
     "matrix_memory": {"kind": "hip", "sources": ["kernels/matrix_memory.hip"], "headers": ["kernels/common.h", "kernels/score_shape.h", "kernels/tanh_norm.h"]},
     "tanh_norm": {"kind": "hip", "sources": ["kernels/tanh_norm.hip"], "headers": ["kernels/common.h", "kernels/score_shape.h", "kernels/tanh_norm.h"]},
     "moe": {"kind": "hip", "sources": ["kernels/moe.hip"], "headers": ["kernels/common.h", "kernels/score_shape.h", "kernels/tanh_norm.h"]},
+    "draft_tree": {"kind": "hip", "sources": ["kernels/draft_tree.hip"], "headers": ["kernels/common.h", "kernels/score_shape.h", "kernels/tanh_norm.h"]},
+    "rotary": {"kind": "hip", "sources": ["kernels/rotary.hip"], "headers": ["kernels/common.h", "kernels/score_shape.h", "kernels/tanh_norm.h"]},
+    "tree_attention": {"kind": "hip", "sources": ["kernels/tree_attention.hip"], "headers": ["kernels/common.h", "kernels/score_shape.h", "kernels/tanh_norm.h"]},
     "sampling": {"kind": "hip", "sources": ["kernels/sampling.hip"],
                  "headers": ["kernels/common.h", "kernels/score_shape.h", "kernels/tanh_norm.h", "kernels/noalloc.h"]},
     "peaks": {"kind": "hip", "sources": ["kernels/peaks.hip"], "headers": ["kernels/common.h", "kernels/score_shape.h", "kernels/tanh_norm.h"]},
@@ -78,14 +81,15 @@ LIBRARIES: Dict[str, dict] = {
     # (host code only; it calls the kernel libraries' entry points)
     "engine": {
         "kind": "hiphost",
-        "sources": ["engine/ops.cc", "engine/ops_sequence.cc", "engine/ops_scored.cc", "engine/parts.cc", "engine/parts_gated.cc",
+        "sources": ["engine/ops.cc", "engine/ops_sequence.cc", "engine/ops_scored.cc", "engine/ops_tree.cc", "engine/parts.cc", "engine/parts_gated.cc",
                     "engine/mamba2.cc", "engine/latent_attention.cc", "engine/scored_attention.cc", "engine/recurrent_parts.cc", "engine/linear_attention.cc", "engine/matrix_memory.cc", "engine/tanh_norm.cc",
                     "engine/json.cc", "engine/weights.cc", "engine/arch.cc",
                     "engine/gpt2.cc", "engine/kugulorn.cc", "engine/rekirax.cc", "engine/viladra.cc", "engine/sunulorn.cc", "engine/zokunex.cc", "engine/gisedra.cc", "engine/engine.cc", "engine/engine_api.cc"],
         "headers": ["kernels/score_shape.h", "kernels/tanh_norm.h", "engine/ops.h", "engine/parts.h", "engine/kernels.h", "engine/json.h", "engine/weights.h",
                     "engine/arch.h", "engine/engine.h", "runtime/cache_manager.h", "runtime/scheduler.h"],
         "needs": ["elementwise", "gemm_f32", "gemm_bf16", "attention", "attention_decode", "attention_prefill",
-                  "norm_gate", "ssm", "latent_attention", "scored_attention", "gated_recurrence", "matrix_memory", "moe", "tanh_norm", "sampling", "runtime"],
+                  "norm_gate", "ssm", "latent_attention", "scored_attention", "gated_recurrence", "matrix_memory", "moe", "tanh_norm",
+                  "draft_tree", "rotary", "tree_attention", "sampling", "runtime"],
     },
     # the command line: a program, not a library (mini_llm_amd/_lib/mini-llm; bin/mini-llm starts it)
     "cli": {

@@ -183,6 +183,18 @@ int mllm_op_token_side(const Tensor2* x, const Tensor2* xb, const Tensor2* gate,
         if (hipStreamSynchronize(s) != hipSuccess) fail("token_side: the kernel failed");
     });
 }
+int mllm_op_tree_max_nodes(void) { return tree_max_nodes(); }
+int mllm_op_step_maps(const StepMapsArgs* a, hipStream_t s) { return guarded([&] { step_maps(*a, s); }); }
+int mllm_op_rotary(const Tensor2* x, const int* positions, const unsigned long long* turns, int pairs, int n_heads, int head_dim, int interleaved,
+                   float amplitude, const Tensor2* out, hipStream_t s) {
+    return guarded([&] { rotary(*x, positions, turns, pairs, n_heads, head_dim, interleaved != 0, amplitude, *out, s); });
+}
+// *floats: what a call with these arguments needs in a->workspace
+int mllm_op_tree_attention_workspace(const TreeAttentionArgs* a, unsigned long long* floats) {
+    return guarded([&] { *floats = tree_attention_workspace_floats(*a); });
+}
+int mllm_op_tree_attention(const TreeAttentionArgs* a, hipStream_t s) { return guarded([&] { tree_attention(*a, s); }); }
+int mllm_op_tree_accept(const TreeAcceptArgs* a, hipStream_t s) { return guarded([&] { tree_accept(*a, s); }); }
 int mllm_op_argmax(const Tensor2* logits, int* out, hipStream_t s) { return guarded([&] { argmax(*logits, out, s); }); }
 int mllm_op_sample(const Tensor2* logits, const float* temperature, const float* u, int* out, hipStream_t s) {
     return guarded([&] { sample(*logits, temperature, u, out, s); });

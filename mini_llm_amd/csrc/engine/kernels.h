@@ -211,4 +211,20 @@ int mllm_argmax_mirrored(const float* logits, int ld, int n, int V, int* out, in
 int mllm_sample_mirrored(const float* logits, int ld, int n, int V, const float* temperature, const float* u, int* out, int* mirror,
                 hipStream_t stream);
 
+// draft_tree.hip, rotary.hip, tree_attention.hip
+int mllm_tree_max_nodes(void);
+int mllm_step_maps(const int* rows, const int* n_new, const int* lengths, const int* pages, long long ld_pages, const int* parents, int n_seqs,
+                   int n_requests, int tokens, int page_size, int n_pages, int max_blocks, int max_new, int words, int* cu_q, int* cached,
+                   int* ctx_len, int* token_seq, int* positions, int* slots, int* block_tables, unsigned long long* ancestors, hipStream_t stream);
+int mllm_tree_accept(const int* choices, const int* ids, const int* parents, const int* cu_q, const int* cached, const int* block_tables,
+                     const int* rows, int n_seqs, int tokens, int page_size, int n_pages, int max_blocks, int max_new, int n_requests, int* kept,
+                     int* path, int* next, int* slots, int* lengths, hipStream_t stream);
+int mllm_rotary(const void* x, long long ldx, const int* positions, const unsigned long long* turns, int tokens, int pairs, int n_heads,
+                int head_dim, int interleaved, float amplitude, void* out, long long ldo, int dtype, hipStream_t stream);
+long long mllm_tree_attention_ws_floats(int tokens, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_new, int max_cached, int window, int dtype);
+int mllm_tree_attention(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* k_pages, const void* v_pages,
+                        int n_pages, int page_size, const int* block_tables, int n_seqs, int max_blocks, const int* cached, const int* cu_q,
+                        const unsigned long long* ancestors, int words, const int* positions, int tokens, int n_heads, int n_kv_heads, int head_dim,
+                        float scale, int window, int max_new, int max_cached, void* out, long long ldo, float* ws, int dtype, hipStream_t stream);
+
 }  // extern "C"

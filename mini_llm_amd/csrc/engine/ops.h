@@ -491,6 +491,63 @@ void concat_cast(const Tensor2& a, const Tensor2& b, const Tensor2& out, hipStre
 // out[t, j] = act(gu[t, j]) * gu[t, F + j] (act: GELU_TANH or GLU_SILU)
 void glu_act(const Tensor2& gu, int act, const Tensor2& out, hipStream_t stream);
 
+// -- trees of drafted tokens -------------------------------------------------------------------------
+// A step in which every sequence brings several tokens that need not follow one another: a tree of drafted tokens whose node i has
+// parent parents[i] < i within its sequence (-1: a root). step_maps makes the step's arrays, rotary turns queries and keys by its
+// positions, tree_attention reads the cache, and with the token that the model chose at every node tree_accept finds what stands; kv_append
+// then writes the kept nodes' keys and values to the slots it gives. All of it stays on the device, so that the next step can be
+// launched without the host having seen the result of this one.
+//
+// rows[b] (null: b): the request's row of lengths, pages (a place without a request: a row outside them). cu_q [n_seqs + 1], cached and
+// ctx_len (cached + new) [n_seqs], token_seq, positions and slots (page rows) [tokens], block_tables [n_seqs, max_blocks] with the pages
+// of ctx_len positions and zeros behind them. With parents: positions are cached + depth, slots are -1, and ancestors [tokens, words] has bit i % 64 of
+// word i / 64 set for the node itself and every node above it. A sequence has at most max_new tokens (more are left out), all together
+// at most `tokens`; the tokens behind the last sequence get sequence 0, position 0, slot -1 and no ancestors.
+struct StepMapsArgs {
+    const int *rows = nullptr, *n_new = nullptr, *lengths = nullptr, *pages = nullptr, *parents = nullptr;
+    int64_t ld_pages = 0;
+    int n_seqs = 0, n_requests = 0, tokens = 0, page_size = 0, n_pages = 0, max_blocks = 0, max_new = 0, words = 0;
+    int *cu_q = nullptr, *cached = nullptr, *ctx_len = nullptr, *token_seq = nullptr, *positions = nullptr, *slots = nullptr, *block_tables = nullptr;
+    unsigned long long* ancestors = nullptr;
+};
+int tree_max_nodes();
+void step_maps(const StepMapsArgs& a, hipStream_t stream);
+// out = x [T, n_heads * head_dim] with the first 2 * pairs columns of every head turned by positions[t] * turns[i] (64-bit shares of a
+// turn), as halves (i, i + pairs) or neighbours (2i, 2i + 1), times amplitude; the columns behind as they are. out may be x.
+void rotary(const Tensor2& x, const int* positions, const unsigned long long* turns, int pairs, int n_heads, int head_dim, bool interleaved,
+            float amplitude, const Tensor2& out, hipStream_t stream);
+struct TreeAttentionArgs {
+    Tensor2 q, k, v;                       // the step's rows: [T, n_heads * head_dim], [T, n_kv_heads * head_dim] twice (any row strides)
+    int n_heads = 0, n_kv_heads = 0, head_dim = 0;
+    Tensor2 k_pages, v_pages;              // [n_pages * page_size, n_kv_heads * head_dim]
+    int page_size = 0;
+    const int* block_tables = nullptr;     // [n_seqs, max_blocks]
+    int n_seqs = 0, max_blocks = 0;
+    const int* cached = nullptr;           // [n_seqs]
+    const int* cu_q = nullptr;             // [n_seqs + 1]
+    const unsigned long long* ancestors = nullptr;      // [T, words]
+    int words = 0;
+    const int* positions = nullptr;        // [T] (with a window)
+    float scale = 1.f;
+    int window = 0;
+    int max_new = 0, max_cached = 0;       // no sequence brings more nodes; the longest cache (the choice of splits goes by it)
+    Tensor2 out;                           // [T, n_heads * head_dim]
+    float* workspace = nullptr;
+    size_t workspace_floats = 0;
+};
+// Rows that see nothing are zeros; rows of no sequence stay as they are.
+void tree_attention(const TreeAttentionArgs& a, hipStream_t stream);
+size_t tree_attention_workspace_floats(const TreeAttentionArgs& a);
+// choices[t]: the token chosen at node t, ids[t]: its drafted token. From the first node of a sequence on, to the first child whose token was
+// chosen: kept [n_seqs] nodes, their rows path [n_seqs, max_new] (-1 behind them), the token chosen at the last one, the page rows of
+// the kept nodes' keys and values, slots [tokens] (-1: not kept), and lengths[rows[b]] = cached[b] + kept[b] (lengths may be null).
+struct TreeAcceptArgs {
+    const int *choices = nullptr, *ids = nullptr, *parents = nullptr, *cu_q = nullptr, *cached = nullptr, *block_tables = nullptr, *rows = nullptr;
+    int n_seqs = 0, tokens = 0, page_size = 0, n_pages = 0, max_blocks = 0, max_new = 0, n_requests = 0;
+    int *kept = nullptr, *path = nullptr, *next = nullptr, *slots = nullptr, *lengths = nullptr;
+};
+void tree_accept(const TreeAcceptArgs& a, hipStream_t stream);
+
 // `mirror` (optional): a second place for the chosen tokens, which may be pinned host memory (the kernel that
 // chooses writes it: no copy has to be launched for the host to read them).
 void argmax(const Tensor2& logits, int* out, hipStream_t stream, int* mirror = nullptr);

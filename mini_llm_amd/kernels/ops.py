@@ -9,6 +9,7 @@ loaded, raises.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional
 
 import torch
@@ -60,6 +61,25 @@ class TanhNormC(ctypes.Structure):
     _fields_ = [("alpha", _vp), ("weight", _vp), ("bias", _vp)]
 
 
+class StepMapsC(ctypes.Structure):
+    _fields_ = [(n, _vp) for n in ("rows", "n_new", "lengths", "pages", "parents")] + [("ld_pages", _i64)] + \
+               [(n, _i) for n in ("n_seqs", "n_requests", "tokens", "page_size", "n_pages", "max_blocks", "max_new", "words")] + \
+               [(n, _vp) for n in ("cu_q", "cached", "ctx_len", "token_seq", "positions", "slots", "block_tables", "ancestors")]
+
+
+class TreeAttentionC(ctypes.Structure):
+    _fields_ = [("q", Tensor2), ("k", Tensor2), ("v", Tensor2), ("n_heads", _i), ("n_kv_heads", _i), ("head_dim", _i), ("k_pages", Tensor2),
+                ("v_pages", Tensor2), ("page_size", _i), ("block_tables", _vp), ("n_seqs", _i), ("max_blocks", _i), ("cached", _vp), ("cu_q", _vp),
+                ("ancestors", _vp), ("words", _i), ("positions", _vp), ("scale", _f), ("window", _i), ("max_new", _i), ("max_cached", _i),
+                ("out", Tensor2), ("workspace", _vp), ("workspace_floats", ctypes.c_size_t)]
+
+
+class TreeAcceptC(ctypes.Structure):
+    _fields_ = [(n, _vp) for n in ("choices", "ids", "parents", "cu_q", "cached", "block_tables", "rows")] + \
+               [(n, _i) for n in ("n_seqs", "tokens", "page_size", "n_pages", "max_blocks", "max_new", "n_requests")] + \
+               [(n, _vp) for n in ("kept", "path", "next", "slots", "lengths")]
+
+
 _lib = None
 
 
@@ -86,6 +106,12 @@ def engine_library():
         "mllm_op_stream_add": (_i, [T2p, T2p, T2p, _vp, T2p, ctypes.POINTER(TanhNormC), ctypes.POINTER(TanhNormC), _i, _vp]),
         "mllm_op_linear_stream_add": (_i, [T2p, T2p, _vp, T2p, T2p, T2p, ctypes.POINTER(TanhNormC), ctypes.POINTER(TanhNormC), _vp]),
         "mllm_op_token_side": (_i, [T2p, T2p, T2p, T2p, _vp, _f, _vp, _vp, _vp, _i, T2p, _i, T2p, ctypes.POINTER(TanhNormC), _vp]),
+        "mllm_op_tree_max_nodes": (_i, []),
+        "mllm_op_step_maps": (_i, [ctypes.POINTER(StepMapsC), _vp]),
+        "mllm_op_rotary": (_i, [T2p, _vp, _vp, _i, _i, _i, _i, _f, T2p, _vp]),
+        "mllm_op_tree_attention_workspace": (_i, [ctypes.POINTER(TreeAttentionC), ctypes.POINTER(ctypes.c_ulonglong)]),
+        "mllm_op_tree_attention": (_i, [ctypes.POINTER(TreeAttentionC), _vp]),
+        "mllm_op_tree_accept": (_i, [ctypes.POINTER(TreeAcceptC), _vp]),
         "mllm_op_argmax": (_i, [T2p, _vp, _vp]),
         "mllm_op_sample": (_i, [T2p, _vp, _vp, _vp, _vp]),
     }
@@ -604,3 +630,223 @@ def token_side(x, xb, gate, proj, weight, eps, ids, table, col0, copy=None, next
     _ok(engine_library().mllm_op_token_side(_ref(x, "x"), _ref(xb, "xb"), _ref(gate, "gate"), _ref(proj, "proj"), _p(weight), eps, _p(ids), _p(src), _p(prev),
                                             0 if prev is None else prev.numel(), _ref(table, "table"), col0, _ref(copy, "copy"), _norm(next), _stream()))
     return x
+
+
+# -- trees of drafted tokens -----------------------------------------------------------------------------
+# A step that has the model check several drafted tokens of a request at once: step_maps, (products, rotary, tree_attention) of every
+# layer, argmax or sample at every node, tree_accept, and kv_append with its slots for every layer. A tree is given by its nodes' parents,
+# numbered within the sequence and standing in front of their children; node 0 is the last token that is certain.
+
+def tree_max_nodes() -> int:
+    """The most nodes of one sequence's tree."""
+    return int(engine_library().mllm_op_tree_max_nodes())
+
+
+def _here(*tensors: Optional[torch.Tensor]) -> None:
+    """All on one GPU, and that the current one (whose current stream the op is launched on)."""
+    _gpu(*tensors)
+    for t in tensors:
+        if t is not None and t.device.index != torch.cuda.current_device():
+            raise KernelError(f"tensor is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _counted(t: torch.Tensor, name: str, n: int) -> None:
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != 1 or t.numel() != n:
+        raise KernelError(f"{name} must be contiguous int32 [{n}], got {tuple(t.shape)} {t.dtype}")
+
+
+def _table(t: torch.Tensor, name: str, rows: Optional[int] = None) -> None:
+    if t.dim() != 2 or t.dtype != torch.int32 or t.shape[0] < 1 or t.shape[1] < 1 or (t.shape[1] > 1 and t.stride(1) != 1) or \
+            (rows is not None and t.shape[0] != rows):
+        raise KernelError(f"{name} must be int32 [{'requests' if rows is None else rows}, blocks] with contiguous rows, got {tuple(t.shape)} {t.dtype}")
+
+
+class StepMaps:
+    """The arrays of a step of ``n_seqs`` sequences and up to ``tokens`` tokens, of which one sequence brings at most ``max_new``:
+    ``cu_q`` [n_seqs + 1], ``cached`` and ``ctx_len`` [n_seqs], ``token_seq``, ``positions`` and ``slots`` [tokens],
+    ``block_tables`` [n_seqs, max_blocks] (int32), and for trees ``ancestors`` [tokens, ceil(max_new / 64)] (int64: bit i % 64 of
+    word i // 64 is set for the node itself and every node above it). Kept by a program from step to step; ``step_maps`` fills it."""
+
+    def __init__(self, n_seqs: int, tokens: int, max_blocks: int, max_new: int, tree: bool = False, device=None):
+        if min(n_seqs, tokens, max_blocks, max_new) < 1:
+            raise KernelError(f"step maps of {n_seqs} sequences, {tokens} tokens, {max_blocks} blocks, {max_new} tokens a sequence")
+        if tree and max_new > tree_max_nodes():
+            raise KernelError(f"a tree has at most {tree_max_nodes()} nodes, not {max_new}")
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+        self.max_new = max_new
+        zeros = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=device)      # noqa: E731
+        self.cu_q, self.cached, self.ctx_len = zeros(n_seqs + 1), zeros(n_seqs), zeros(n_seqs)
+        self.token_seq, self.positions, self.slots = zeros(tokens), zeros(tokens), zeros(tokens)
+        self.block_tables = zeros(n_seqs, max_blocks)
+        self.ancestors = torch.zeros((tokens, (max_new + 63) // 64), dtype=torch.int64, device=device) if tree else None
+
+
+def step_maps(maps: StepMaps, rows: Optional[torch.Tensor], n_new: torch.Tensor, lengths: torch.Tensor, pages: torch.Tensor, page_size: int,
+              n_pages: int, parents: Optional[torch.Tensor] = None) -> StepMaps:
+    """Fills ``maps`` on the device. Sequence b is request rows[b] (``rows`` None: b; a row outside the requests: nobody), which has
+    lengths[r] tokens in the pages pages[r, :] and brings n_new[b] more. All int32: n_new (and rows) [n_seqs], lengths [requests], pages
+    [requests, >= max_blocks] (any row stride).
+
+    Without ``parents`` the tokens follow one another: positions from lengths[r] on, slots their page rows. With ``parents`` (int32
+    [tokens], needs maps made with ``tree=True``) they are a tree each: positions are lengths[r] + depth, slots -1 (``tree_accept``
+    says later where the kept ones go), ancestors the sets that ``tree_attention`` takes; a parent that does not stand in front of its
+    child counts as none. More than ``max_new`` tokens of a sequence, or more than ``tokens`` together, are left out (cu_q says how
+    many are in). A position beyond ``max_blocks``, or whose page is none of the ``n_pages``, has slot -1. Tokens behind the last sequence get
+    sequence 0, position 0, slot -1 and no ancestors."""
+    B, T, blocks = maps.cached.numel(), maps.token_seq.numel(), maps.block_tables.shape[1]
+    _counted(n_new, "n_new", B)
+    if rows is not None:
+        _counted(rows, "rows", B)
+    _table(pages, "pages")
+    if pages.shape[1] < blocks:
+        raise KernelError(f"pages has {pages.shape[1]} blocks a request, the maps {blocks}")
+    _counted(lengths, "lengths", pages.shape[0])
+    if parents is not None:
+        if maps.ancestors is None:
+            raise KernelError("parents need step maps made for trees")
+        _counted(parents, "parents", T)
+    _here(rows, n_new, lengths, pages, parents, maps.cu_q)
+    a = StepMapsC(rows=None if rows is None else rows.data_ptr(), n_new=n_new.data_ptr(), lengths=lengths.data_ptr(), pages=pages.data_ptr(),
+                  parents=None if parents is None else parents.data_ptr(), ld_pages=pages.stride(0) if pages.shape[0] > 1 else pages.shape[1], n_seqs=B,
+                  n_requests=pages.shape[0], tokens=T, page_size=int(page_size), n_pages=int(n_pages), max_blocks=blocks, max_new=maps.max_new,
+                  words=0 if parents is None else maps.ancestors.shape[1], cu_q=maps.cu_q.data_ptr(), cached=maps.cached.data_ptr(),
+                  ctx_len=maps.ctx_len.data_ptr(), token_seq=maps.token_seq.data_ptr(), positions=maps.positions.data_ptr(), slots=maps.slots.data_ptr(),
+                  block_tables=maps.block_tables.data_ptr(), ancestors=None if parents is None else maps.ancestors.data_ptr())
+    _ok(engine_library().mllm_op_step_maps(ctypes.byref(a), _stream()))
+    return maps
+
+
+def rotary_freqs(rot_dims: int, base: float = 10000.0, scaling: Optional[dict] = None, device=None) -> torch.Tensor:
+    """What ``rotary`` turns by: for every pair of the first ``rot_dims`` columns its share of a turn per position, in 64 bits of
+    fixed point (int64 [rot_dims / 2]). Pair i turns by f_i = base^(-2i / rot_dims) radians a position, or, for contexts longer than
+    those of training, with ``scaling``:
+
+    * ``{"kind": "linear", "factor": s}``: f_i / s;
+    * ``{"kind": "base", "factor": s}``: base * s^(rot_dims / (rot_dims - 2)) as the base, so that the slowest pair is slowed by s and the
+      fastest not at all;
+    * ``{"kind": "by_turns", "factor": s, "original": n, "fast": f, "slow": w}``: f_i where the pair makes at least f turns over the n
+      positions of training, f_i / s where it makes at most w, between them the mixture that is linear in its turns;
+    * ``{"kind": "by_pair", ...}`` (the same numbers): the mixture linear in the pair's number, between the (fractional) pairs that make f and w turns."""
+    if rot_dims < 2 or rot_dims % 2 or not base > 0.0 or not math.isfinite(base):
+        raise KernelError(f"rotary positions of {rot_dims} columns with base {base}: columns come in pairs, the base is positive")
+    kind = None if scaling is None else scaling.get("kind")
+    if kind not in (None, "linear", "base", "by_turns", "by_pair"):
+        raise KernelError(f"unknown scaling of rotary positions '{kind}'")
+    numbers = {"linear": ("factor",), "base": ("factor",), None: ()}.get(kind, ("factor", "original", "fast", "slow"))
+    if scaling is not None and set(scaling) != {"kind", *numbers}:
+        raise KernelError(f"scaling '{kind}' takes {', '.join(numbers)}, got {sorted(scaling)}")
+    s = float(scaling["factor"]) if kind else 1.0
+    if not s > 0.0 or not math.isfinite(s):
+        raise KernelError(f"scaling factor {s}: a positive number is needed")
+    if kind == "base":
+        if rot_dims < 4:
+            raise KernelError("scaling 'base' needs at least two pairs")
+        base = base * s ** (rot_dims / (rot_dims - 2))
+    freqs = [base ** (-2.0 * i / rot_dims) for i in range(rot_dims // 2)]
+    if kind == "linear":
+        freqs = [f / s for f in freqs]
+    if kind in ("by_turns", "by_pair"):
+        n, fast, slow = (float(scaling[x]) for x in ("original", "fast", "slow"))
+        if not (n > 0.0 and fast > slow > 0.0 and math.isfinite(n) and math.isfinite(fast)) or (kind == "by_pair" and not base > 1.0):
+            raise KernelError(f"scaling '{kind}': original {n}, fast {fast} and slow {slow} turns (fast > slow > 0)")
+        if kind == "by_turns":
+            keep = [(n * f / (2.0 * math.pi) - slow) / (fast - slow) for f in freqs]
+        else:
+            at = lambda turns: rot_dims * math.log(n / (2.0 * math.pi * turns)) / (2.0 * math.log(base))      # noqa: E731 (the pair that makes so many)
+            keep = [1.0 - (i - at(fast)) / (at(slow) - at(fast)) for i in range(len(freqs))]
+        keep = [min(1.0, max(0.0, k)) for k in keep]
+        freqs = [k * f + (1.0 - k) * f / s for k, f in zip(keep, freqs)]
+    shares = [int(math.fmod(f / (2.0 * math.pi), 1.0) * 2.0 ** 64) % 2 ** 64 for f in freqs]
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+    return torch.tensor([x - 2 ** 64 if x >= 2 ** 63 else x for x in shares], dtype=torch.int64, device=device)
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, n_heads: int, head_dim: int, out: torch.Tensor, interleaved: bool = False,
+           amplitude: float = 1.0) -> torch.Tensor:
+    """out = x [T, n_heads * head_dim] (float32 or bfloat16, any row stride) with pair i < len(freqs) of every head turned by the angle
+    positions[t] * freqs[i] (``rotary_freqs``) and multiplied by ``amplitude``; pairs are columns i and i + len(freqs) of a head, or 2i and
+    2i + 1 with ``interleaved``; the columns behind them are handed on. ``out`` may be ``x``. positions: int32 [T], in any order; angles
+    are exact to 2^-32 of a turn at any of them."""
+    if freqs.dim() != 1 or freqs.dtype != torch.int64 or not freqs.is_contiguous() or freqs.numel() < 1:
+        raise KernelError("freqs must be contiguous int64 [pairs] (rotary_freqs)")
+    if x.dim() != 2 or x.shape != out.shape:
+        raise KernelError(f"rotary: x {tuple(x.shape)} and out {tuple(out.shape)} must be [T, n_heads * head_dim]")
+    _counted(positions, "positions", x.shape[0])
+    tx, to = t2(x, "x"), t2(out, "out")
+    _here(x, positions, freqs, out)
+    _ok(engine_library().mllm_op_rotary(ctypes.byref(tx), _p(positions), _p(freqs), freqs.numel(), int(n_heads), int(head_dim), 1 if interleaved else 0,
+                                        float(amplitude), ctypes.byref(to), _stream()))
+    return out
+
+
+def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, k_pages: torch.Tensor,
+                   v_pages: torch.Tensor, page_size: int, block_tables: torch.Tensor, cached: torch.Tensor, cu_q: torch.Tensor, ancestors: torch.Tensor,
+                   positions: Optional[torch.Tensor], scale: float, out: torch.Tensor, *, max_new: int, max_cached: int, window: int = 0) -> torch.Tensor:
+    """Attention of drafted trees. Node t of sequence b (rows cu_q[b] to cu_q[b + 1]) sees the cached[b] positions in the pages and, of
+    its own sequence's nodes, those whose bit is set in ancestors[t] (``StepMaps``; its own bit among them, or it does not see
+    itself); their keys and values are rows of ``k`` and ``v`` and need not be in the pages. With a window, what stands at positions[t] -
+    window or in front of it is not seen.
+
+    q: [T, n_heads * head_dim], k, v: [T, n_kv_heads * head_dim] (float32 or bfloat16; rows 16-byte aligned, any strides: columns of the
+    projection's rows), head_dim a multiple of 8 up to 256, out like q, apart from the inputs. block_tables: int32 [n_seqs, max_blocks], cached [n_seqs], cu_q
+    [n_seqs + 1], ancestors int64 [T, words], positions [T] (only with a window). No sequence brings more than ``max_new`` <= 64 * words nodes
+    (those beyond are not computed); ``max_cached``, the longest cache, decides how the keys are shared out. A node that sees nothing gets zeros;
+    rows of no sequence stay as they are; what is not seen counts for nothing, NaN among it; a table's entry that names no page holds nothing."""
+    T, B = q.shape[0], cached.numel()
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or not block_tables.is_contiguous() or block_tables.shape[0] != B or block_tables.shape[1] < 1:
+        raise KernelError(f"block_tables must be contiguous int32 [{B}, max_blocks]")
+    _counted(cached, "cached", B)
+    _counted(cu_q, "cu_q", B + 1)
+    if ancestors.dim() != 2 or ancestors.dtype != torch.int64 or not ancestors.is_contiguous() or ancestors.shape[0] != T:
+        raise KernelError(f"ancestors must be contiguous int64 [{T}, words]")
+    if window and positions is None:
+        raise KernelError("tree_attention: positions are needed with a window")
+    if positions is not None:
+        _counted(positions, "positions", T)
+    a = TreeAttentionC()
+    a.q, a.k, a.v, a.k_pages, a.v_pages, a.out = (t2(t, n) for t, n in ((q, "q"), (k, "k"), (v, "v"), (k_pages, "k_pages"), (v_pages, "v_pages"), (out, "out")))
+    _here(q, k, v, k_pages, v_pages, block_tables, cached, cu_q, ancestors, positions, out)
+    a.n_heads, a.n_kv_heads, a.head_dim, a.page_size = int(n_heads), int(n_kv_heads), int(head_dim), int(page_size)
+    a.block_tables, a.n_seqs, a.max_blocks = block_tables.data_ptr(), B, block_tables.shape[1]
+    a.cached, a.cu_q, a.ancestors, a.words = cached.data_ptr(), cu_q.data_ptr(), ancestors.data_ptr(), ancestors.shape[1]
+    a.positions = None if positions is None else positions.data_ptr()
+    a.scale, a.window, a.max_new, a.max_cached = float(scale), int(window or 0), int(max_new), int(max_cached)
+    lib, floats = engine_library(), ctypes.c_ulonglong(0)
+    _ok(lib.mllm_op_tree_attention_workspace(ctypes.byref(a), ctypes.byref(floats)))
+    if floats.value:
+        # (of the caller's stream and, in a capture, of the graph's own pool: two graphs share none)
+        ws = torch.empty(floats.value, dtype=torch.float32, device=q.device)
+        a.workspace, a.workspace_floats = ws.data_ptr(), floats.value
+    _ok(lib.mllm_op_tree_attention(ctypes.byref(a), _stream()))
+    return out
+
+
+def tree_accept(choices: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor, cu_q: torch.Tensor, cached: torch.Tensor, block_tables: torch.Tensor,
+                page_size: int, n_pages: int, kept: torch.Tensor, path: torch.Tensor, next_token: torch.Tensor, slots: torch.Tensor,
+                lengths: Optional[torch.Tensor] = None, rows: Optional[torch.Tensor] = None) -> None:
+    """What stands of the drafted trees. choices[t] is the token that the model chose at node t (``argmax``, or ``sample``, whose
+    distribution the kept tokens then have), ids[t] the node's drafted token. A sequence's first node stands; after a node that stands, the first
+    of its children whose token was chosen at it does. Writes, all int32: kept [n_seqs], the number of nodes that stand; path [n_seqs, max_new],
+    their rows, -1 behind them; next_token [n_seqs], the choice at the last (a sequence without nodes: 0, -1, -1); slots [T], the page row of
+    each node that stands (position cached[b] + its place on the path), -1 for the others and the rows of no sequence: what ``kv_append`` takes.
+    With ``lengths`` (int32 [requests]): lengths[rows[b]] = cached[b] + kept[b] (``rows`` None: b). A page that is none of the ``n_pages`` gives slot -1."""
+    T, B = choices.numel(), cached.numel()
+    for t, n in ((choices, "choices"), (ids, "ids"), (parents, "parents"), (slots, "slots")):
+        _counted(t, n, T)
+    for t, n in ((cached, "cached"), (kept, "kept"), (next_token, "next_token")):
+        _counted(t, n, B)
+    _counted(cu_q, "cu_q", B + 1)
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or not block_tables.is_contiguous() or block_tables.shape[0] != B or block_tables.shape[1] < 1:
+        raise KernelError(f"block_tables must be contiguous int32 [{B}, max_blocks]")
+    if path.dim() != 2 or path.dtype != torch.int32 or not path.is_contiguous() or path.shape[0] != B or path.shape[1] < 1:
+        raise KernelError(f"path must be contiguous int32 [{B}, max_new]")
+    if rows is not None:
+        _counted(rows, "rows", B)
+    if lengths is not None:
+        _counted(lengths, "lengths", lengths.numel() if rows is not None else B)
+    _here(choices, ids, parents, cu_q, cached, block_tables, kept, path, next_token, slots, lengths, rows)
+    ptr = lambda t: None if t is None else t.data_ptr()      # noqa: E731
+    a = TreeAcceptC(choices=ptr(choices), ids=ptr(ids), parents=ptr(parents), cu_q=ptr(cu_q), cached=ptr(cached), block_tables=ptr(block_tables), rows=ptr(rows),
+                    n_seqs=B, tokens=T, page_size=int(page_size), n_pages=int(n_pages), max_blocks=block_tables.shape[1], max_new=path.shape[1],
+                    n_requests=0 if lengths is None else lengths.numel(), kept=ptr(kept), path=ptr(path), next=ptr(next_token), slots=ptr(slots), lengths=ptr(lengths))
+    _ok(engine_library().mllm_op_tree_accept(ctypes.byref(a), _stream()))
