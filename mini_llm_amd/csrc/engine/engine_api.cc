@@ -189,9 +189,11 @@ int mllm_op_rotary(const Tensor2* x, const int* positions, const unsigned long l
                    float amplitude, const Tensor2* out, hipStream_t s) {
     return guarded([&] { rotary(*x, positions, turns, pairs, n_heads, head_dim, interleaved != 0, amplitude, *out, s); });
 }
-// *floats: what a call with these arguments needs in a->workspace
-int mllm_op_tree_attention_workspace(const TreeAttentionArgs* a, unsigned long long* floats) {
-    return guarded([&] { *floats = tree_attention_workspace_floats(*a); });
+// Floats of workspace that a call of these sizes needs (0 for sizes that the call itself refuses)
+long long mllm_op_tree_attention_workspace(int tokens, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_new, int max_cached, int window, int dtype) {
+    long long floats = 0;
+    guarded([&] { floats = static_cast<long long>(tree_attention_workspace_floats(tokens, n_seqs, n_heads, n_kv_heads, head_dim, max_new, max_cached, window, dtype)); });
+    return floats;
 }
 int mllm_op_tree_attention(const TreeAttentionArgs* a, hipStream_t s) { return guarded([&] { tree_attention(*a, s); }); }
 int mllm_op_tree_accept(const TreeAcceptArgs* a, hipStream_t s) { return guarded([&] { tree_accept(*a, s); }); }

@@ -537,7 +537,8 @@ struct TreeAttentionArgs {
 };
 // Rows that see nothing are zeros; rows of no sequence stay as they are.
 void tree_attention(const TreeAttentionArgs& a, hipStream_t stream);
-size_t tree_attention_workspace_floats(const TreeAttentionArgs& a);
+// (0 for sizes that tree_attention refuses)
+size_t tree_attention_workspace_floats(int tokens, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_new, int max_cached, int window, int dtype);
 // choices[t]: the token chosen at node t, ids[t]: its drafted token. From the first node of a sequence on, to the first child whose token was
 // chosen: kept [n_seqs] nodes, their rows path [n_seqs, max_new] (-1 behind them), the token chosen at the last one, the page rows of
 // the kept nodes' keys and values, slots [tokens] (-1: not kept), and lengths[rows[b]] = cached[b] + kept[b] (lengths may be null).

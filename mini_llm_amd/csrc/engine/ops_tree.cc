@@ -91,14 +91,16 @@ static void check_tree_attention(const TreeAttentionArgs& a) {
         if (overlap(a.out, *t)) fail("tree_attention: out shares memory with an input");
 }
 
-size_t tree_attention_workspace_floats(const TreeAttentionArgs& a) {
-    check_tree_attention(a);
-    return static_cast<size_t>(mllm_tree_attention_ws_floats(static_cast<int>(a.q.rows), a.n_seqs, a.n_heads, a.n_kv_heads, a.head_dim, a.max_new, a.max_cached,
-                                                             a.window, a.q.dtype));
+size_t tree_attention_workspace_floats(int tokens, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_new, int max_cached, int window, int dtype) {
+    if (tokens < 1 || n_seqs < 1 || n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads != 0 || head_dim < 8 || head_dim > 256 || max_new < 1 ||
+        max_new > tree_max_nodes() || max_cached < 0 || window < 0) return 0;
+    return static_cast<size_t>(mllm_tree_attention_ws_floats(tokens, n_seqs, n_heads, n_kv_heads, head_dim, max_new, max_cached, window, dtype));
 }
 
 void tree_attention(const TreeAttentionArgs& a, hipStream_t stream) {
-    const size_t floats = tree_attention_workspace_floats(a);
+    check_tree_attention(a);
+    const size_t floats = tree_attention_workspace_floats(static_cast<int>(a.q.rows), a.n_seqs, a.n_heads, a.n_kv_heads, a.head_dim, a.max_new, a.max_cached, a.window,
+                                                          a.q.dtype);
     if (floats > 0 && (a.workspace == nullptr || a.workspace_floats < floats || !aligned(a.workspace, 16)))
         fail("tree_attention: a workspace of %zu floats is needed (16-byte aligned), %zu are there", floats, a.workspace_floats);
     check(mllm_tree_attention(a.q.data, a.q.stride, a.k.data, a.k.stride, a.v.data, a.v.stride, a.k_pages.data, a.v_pages.data,

@@ -6,21 +6,24 @@
 // What is not seen counts for nothing whatever stands there (infinities and NaN among it), and a block table's entry that names no page of
 // the pool holds nothing that is seen.
 //
-// All nodes of a sequence and all query heads of a key/value head read the same keys, so these are the rows of one product: a workgroup
-// has 16 RT of them (row r is node r / group, head r % group of the key head's), and its wavefronts take the key tiles in turn, each
-// with all rows. Keys and values then go from memory straight into the registers that the matrix instructions read, each once a
-// workgroup, and nothing but the few page rows of a tile passes through LDS until the wavefronts' states meet at the end.
+// All nodes of a sequence and all query heads of a key/value head read the same keys, so these are the rows of one product (row r is node r /
+// group, head r % group of the key head's), of which a workgroup has up to 256. Keys and values come through LDS in stages, loaded straight
+// into it several stages ahead, so that what is on its way holds no register: a compute unit has up to 128 KB on its way where registers
+// would hold half of that. A workgroup's wavefronts are row groups x key groups: each has 16 RT rows, and of every stage the keys of its key
+// group; the key groups' states meet in LDS at the end. Few rows: one row group, many key groups, and memory is what bounds it; many rows: a
+// stage is read by all row groups, and the matrix instructions are.
 //
 // As in prompt attention everything is transposed, so that a lane owns one query row of each 16:
-//   S^T = K Q^T   the lane with row c, group G (lane = 16 G + c) loads key c of each 16, 16 bytes at 64 i + 16 G of its row: the product's k
+//   S^T = K Q^T   the lane with row c, group G (lane = 16 G + c) takes key c of each 16, 16 bytes at 64 i + 16 G of its row: the product's k
 //                 index runs over the columns in an order of its own, the same for queries and keys;
 //   O^T = V^T P^T the lane has the weights of keys 4 G .. 4 G + 3 of each 16 from the first product, in the place where the second wants
-//                 them. As the other operand it loads, of just these keys, 16 (8, 4) bytes at the same place c of a block of 256 (128, 64) bytes:
-//                 column m of the product's tile x is column E m + x of the block, E elements to 16 bytes. In 32 bits the loaded words are
+//                 them. As the other operand it takes, of just these keys, 16 (8, 4) bytes at the same place c of a block of 256 (128, 64) bytes:
+//                 column m of the product's tile x is column E m + x of the block, E elements to 16 bytes. In 32 bits the words are
 //                 the operand; in bfloat16 a byte permutation joins two keys' halves, one instruction a register, shared by all rows.
 // Softmax statistics, sums and outputs are fp32; the weights are rounded to the values' type for the second product (in bfloat16: by half a step,
 // which averages over the keys; the sum is over the weights before they are rounded).
 #include "common.h"
+#include "lds_loads.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -75,156 +78,70 @@ __device__ __forceinline__ uint32_t sifted(uint32_t w, int kind, bf16_t) {
     return (special & (kind == 1 ? mantissa : ~mantissa & (kind == 2 ? ~sign : sign))) * 0x3f80u;
 }
 
-template <typename T, int NT, int RT, int MAXW>
-__global__ void __launch_bounds__(MAXW * 64) tree_attention_kernel(TreeAttentionParams a) {
+// One wavefront's rows, 16 RT of them, and what it has summed up for them.
+template <typename T, int NT, int RT>
+struct Rows {
     using S = Shape<T, NT>;
-    constexpr int KT = S::KT, KEYS = S::KEYS, CH = S::CH, TILES = S::TILES, DIMS = 32 * NT, PITCH = DIMS + 4;
-    extern __shared__ __attribute__((aligned(16))) float state_s[];       // [wavefront][16 RT][PITCH], then maxima and sums
-    __shared__ int row_s[MAXW][KEYS];
+    static constexpr int KT = S::KT, KEYS = S::KEYS, CH = S::CH, TILES = S::TILES;
+    static constexpr unsigned ALL = KEYS == 32 ? 0xffffffffu : 0xffffu;
 
-    // Workgroups that share keys have numbers 8 apart, so that they run on one XCD and the second finds the keys in its L2.
-    const int residue = blockIdx.x % 8, rest = blockIdx.x / 8;
-    const int unit = rest / a.row_tiles * 8 + residue, row_tile = rest % a.row_tiles;
-    if (unit >= a.units) return;
-    const int split = unit % a.nsplit, hk = unit / a.nsplit % a.n_kv_heads, b = unit / a.nsplit / a.n_kv_heads;
-    const int group = a.n_heads / a.n_kv_heads;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, n_waves = blockDim.x / 64;
-    const int G = lane / 16, c16 = lane % 16;
-
-    const int first = min(max(a.cu_q[b], 0), a.tokens);
-    const int nodes = min(min(max(a.cu_q[b + 1] - first, 0), a.tokens - first), a.max_new);
-    const int rows = nodes * group, row0 = row_tile * 16 * RT;
-    if (row0 >= rows) return;
-    const int cached = static_cast<int>(min(min(static_cast<long long>(max(a.cached[b], 0)), static_cast<long long>(a.max_blocks) * a.page_size), INT32_MAX - 64ll));
-    const int row_bytes = a.head_dim * static_cast<int>(sizeof(T));
-    const int* table = a.block_tables + static_cast<size_t>(b) * a.max_blocks;
-
-    // The lane's query row of each 16 (beyond the last: zeros, never written).
     uint4 q[RT][CH];
-    int low[RT], token[RT];
-    int low_least = INT32_MAX, low_most = INT32_MIN;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int r = min(row0 + 16 * rt + c16, rows - 1), node = r / group;
-        token[rt] = first + node;
-        const char* at = a.q + token[rt] * a.ldq + (hk * group + r - node * group) * row_bytes;
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int off = 64 * c + 16 * G;
-            const bool in = off < row_bytes;
-            q[rt][c] = *reinterpret_cast<const uint4*>(at + (in ? off : 0));
-            if (!in) q[rt][c] = make_uint4(0, 0, 0, 0);
-        }
-        low[rt] = a.window > 0 ? a.positions[token[rt]] - a.window + 1 : INT32_MIN;
-        low_least = min(low_least, low[rt]);
-        low_most = max(low_most, low[rt]);
-    }
-    int first_tile = 0;
-    if (a.window > 0) {
-#pragma unroll
-        for (int off = 1; off < 16; off <<= 1) {
-            low_least = min(low_least, __shfl_xor(low_least, off, 64));
-            low_most = max(low_most, __shfl_xor(low_most, off, 64));
-        }
-        low_least = __builtin_amdgcn_readfirstlane(low_least);
-        low_most = __builtin_amdgcn_readfirstlane(low_most);
-        first_tile = min(max(low_least, 0), cached) / KEYS;
-    }
-
-    // Tiles: those of the cache from first_tile on, then the nodes'. A split has `per` neighbouring ones.
-    const int cache_tiles = (cached + KEYS - 1) / KEYS - first_tile, all_tiles = cache_tiles + (nodes + KEYS - 1) / KEYS;
-    const int per = (all_tiles + a.nsplit - 1) / a.nsplit, begin = split * per, end = min(all_tiles, begin + per);
-    const bool whole_pages = a.page_size % 16 == 0;        // 16 neighbouring keys lie in one page
-
     f32x4 o[TILES][RT];
     float m[RT], ref[RT], l[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        m[rt] = -INFINITY; ref[rt] = 0.f; l[rt] = 0.f;
-#pragma unroll
-        for (int x = 0; x < TILES; ++x) o[x][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    int low[RT], token[RT];            // (what stands in front of `low` is not seen)
+    int low_least, low_most;
 
-    // Asks for the page of this lane's key of a tile (of a tile of nodes, or beyond the last: some entry, not used).
-    const int key = lane % KEYS;
-    auto block_of = [&](int at) { return static_cast<int>((static_cast<unsigned long long>(static_cast<unsigned>(at)) * a.page_magic) >> a.page_shift); };
-    auto ask_entry = [&](int tile) { return table[min(block_of((max(min(tile, cache_tiles - 1), 0) + first_tile) * KEYS + key), a.max_blocks - 1)]; };
-    struct Tile {
-        uint4 k[KT][CH];
-        uint32_t v[4 * KT][CH];
-        unsigned valid;          // a bit a key
-    };
-    const char* k_head = a.k_pages + static_cast<size_t>(hk) * row_bytes;
-    const char* v_head = a.v_pages + static_cast<size_t>(hk) * row_bytes;
-    // Asks for a tile's keys and values. All loads are unconditional (keys that are not seen read some row that exists).
-    auto ask = [&](int tile, int entry, Tile& t) {
-        const bool of_nodes = tile >= cache_tiles;
-        int row;
-        bool there;
-        if (of_nodes) {
-            const int j = (tile - cache_tiles) * KEYS + key;
-            there = j < nodes;
-            row = first + min(j, nodes - 1);
-        } else {
-            const int at = (tile + first_tile) * KEYS + key;
-            there = at < cached && static_cast<unsigned>(entry) < static_cast<unsigned>(a.n_pages);
-            row = there ? entry * a.page_size + at - block_of(at) * a.page_size : 0;
-        }
-        t.valid = static_cast<unsigned>(__ballot(there && lane < KEYS));
-        const char *kb = of_nodes ? a.k + static_cast<size_t>(hk) * row_bytes : k_head, *vb = of_nodes ? a.v + static_cast<size_t>(hk) * row_bytes : v_head;
-        const char *kp[KT], *vp[4 * KT];
-        if (whole_pages && !of_nodes && t.valid == (KEYS == 32 ? 0xffffffffu : 0xffffu)) {
+    // Asks for the rows' queries (beyond the last: the last again, never written).
+    __device__ __forceinline__ void begin(const TreeAttentionParams& a, int first, int rows, int group, int hk, int row0, int row_bytes) {
+        const int G = threadIdx.x % 64 / 16, c16 = threadIdx.x % 16;
+        low_least = INT32_MAX;
+        low_most = INT32_MIN;
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                const size_t base = static_cast<size_t>(__builtin_amdgcn_readlane(row, 16 * kt)) * a.page_pitch;
-                kp[kt] = kb + base + c16 * a.page_pitch;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) vp[4 * kt + i] = vb + base + (4 * G + i) * a.page_pitch;
-            }
-        } else {
-            const size_t k_pitch = of_nodes ? a.ldk : a.page_pitch, v_pitch = of_nodes ? a.ldv : a.page_pitch;
-            if (lane < KEYS) row_s[wave][lane] = row;
-            wave_lds_sync();
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                kp[kt] = kb + row_s[wave][16 * kt + c16] * k_pitch;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) vp[4 * kt + i] = vb + row_s[wave][16 * kt + 4 * G + i] * v_pitch;
-            }
-            wave_lds_sync();
-        }
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+        for (int rt = 0; rt < RT; ++rt) {
+            const int r = min(row0 + 16 * rt + c16, rows - 1), node = r / group;
+            token[rt] = first + node;
+            const char* at = a.q + token[rt] * a.ldq + (hk * group + r - node * group) * row_bytes;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int off = 64 * c + 16 * G;
-                const bool check = 64 * (c + 1) > 32 * S::LEAST * static_cast<int>(sizeof(T));
-                t.k[kt][c] = *reinterpret_cast<const uint4*>(kp[kt] + (!check || off < row_bytes ? off : 0));
+                q[rt][c] = *reinterpret_cast<const uint4*>(at + (off < row_bytes ? off : 0));
             }
+            low[rt] = a.window > 0 ? a.positions[token[rt]] - a.window + 1 : INT32_MIN;
+            low_least = min(low_least, low[rt]);
+            low_most = max(low_most, low[rt]);
+        }
+        if (a.window > 0) {
 #pragma unroll
-        for (int j = 0; j < 4 * KT; ++j)
-#pragma unroll
-            for (int w = 0; w < CH; w += S::block_words(w)) {
-                const int off = 64 * w + 4 * S::block_words(w) * c16;
-                const char* p = vp[j] + (off < row_bytes ? off : 0);
-                if (S::block_words(w) == 4) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(p);
-                    t.v[j][w] = x.x; t.v[j][w + 1] = x.y; t.v[j][w + 2] = x.z; t.v[j][w + 3] = x.w;
-                } else if (S::block_words(w) == 2) {
-                    const uint2 x = *reinterpret_cast<const uint2*>(p);
-                    t.v[j][w] = x.x; t.v[j][w + 1] = x.y;
-                } else {
-                    t.v[j][w] = *reinterpret_cast<const uint32_t*>(p);
-                }
+            for (int off = 1; off < 16; off <<= 1) {
+                low_least = min(low_least, __shfl_xor(low_least, off, 64));
+                low_most = max(low_most, __shfl_xor(low_most, off, 64));
             }
-    };
+            low_least = __builtin_amdgcn_readfirstlane(low_least);
+            low_most = __builtin_amdgcn_readfirstlane(low_most);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            m[rt] = -INFINITY; ref[rt] = 0.f; l[rt] = 0.f;
+#pragma unroll
+            for (int x = 0; x < TILES; ++x) o[x][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    // Columns behind the head's last are zero in queries and keys.
+    static constexpr bool maybe_behind(int c) { return 64 * (c + 1) > 32 * S::LEAST * static_cast<int>(sizeof(T)); }
+    __device__ __forceinline__ void wait_for_queries(int row_bytes) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                if (maybe_behind(c) && 64 * c + 16 * static_cast<int>(threadIdx.x % 64 / 16) >= row_bytes) q[rt][c] = make_uint4(0, 0, 0, 0);
+                asm volatile("" : "+v"(q[rt][c].x), "+v"(q[rt][c].y), "+v"(q[rt][c].z), "+v"(q[rt][c].w));
+            }
+    }
 
-    // The second product: into(x, rt, product) for every tile x of columns and 16 rows. With `sift` of the values' elements of a kind (sifted), and
-    // for kinds 1 to 3 with ones in place of the weights.
-    auto weigh = [&](const uint32_t (&v)[4 * KT][CH], const float (&p)[RT][4 * KT], auto sift, int kind, auto&& into) {
-        constexpr bool SIFT = decltype(sift)::value;
-        auto value = [&](int j, int w) { return SIFT ? sifted(v[j][w], kind, T{}) : v[j][w]; };
-        auto weight = [&](int rt, int j) { return SIFT && kind > 0 ? (p[rt][j] == 0.f ? 0.f : 1.f) : p[rt][j]; };
+    // The second product: into(x, rt, product) for every tile x of columns and 16 rows, of the words word(j, w) of the lane's keys j and the weights
+    // weight(rt, j).
+    template <bool ONE_BY_ONE, typename V, typename W, typename F>
+    __device__ __forceinline__ static void weigh(V&& word, W&& weight, F&& into) {
         if constexpr (sizeof(T) == 2) {
             uint4 pb[RT];
 #pragma unroll
@@ -235,7 +152,7 @@ __global__ void __launch_bounds__(MAXW * 64) tree_attention_kernel(TreeAttention
             for (int w = 0; w < CH; ++w) {
                 uint32_t vw[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) vw[j] = value(j, w);
+                for (int j = 0; j < 8; ++j) vw[j] = word(j, w);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t sel = e == 0 ? 0x05040100u : 0x07060302u;
@@ -247,105 +164,81 @@ __global__ void __launch_bounds__(MAXW * 64) tree_attention_kernel(TreeAttention
                             return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, pb[rt]), c, 0, 0, 0);
                         });
                 }
-                if (SIFT) __builtin_amdgcn_sched_barrier(0);
+                if (ONE_BY_ONE) __builtin_amdgcn_sched_barrier(0);
             }
         } else {
 #pragma unroll
             for (int w = 0; w < CH; ++w) {
+                float vw[4 * KT];
+#pragma unroll
+                for (int j = 0; j < 4 * KT; ++j) vw[j] = __builtin_bit_cast(float, word(j, w));
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
                     into(w, rt, [&](f32x4 c) {
 #pragma unroll
-                        for (int j = 0; j < 4 * KT; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, value(j, w)), weight(rt, j), c, 0, 0, 0);
+                        for (int j = 0; j < 4 * KT; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(vw[j], weight(rt, j), c, 0, 0, 0);
                         return c;
                     });
-                if (SIFT) __builtin_amdgcn_sched_barrier(0);
+                if (ONE_BY_ONE) __builtin_amdgcn_sched_barrier(0);
             }
         }
-    };
+    }
 
-    auto take = [&](int tile, Tile& t) {
-        const bool of_nodes = tile >= cache_tiles;
-        const int at0 = of_nodes ? (tile - cache_tiles) * KEYS : (tile + first_tile) * KEYS;
-        const bool all_seen = !of_nodes && t.valid == (KEYS == 32 ? 0xffffffffu : 0xffffu) && (a.window <= 0 || at0 >= low_most);
-        // (columns behind the head's last: zero on both sides)
+    // The scores of a tile's keys, in base 2. keys(kt, k) gives the lane's operands.
+    template <typename K>
+    __device__ __forceinline__ void scores(float (&p)[RT][4 * KT], float scale_log2e, int row_bytes, K&& keys) const {
+        const int G = threadIdx.x % 64 / 16;
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+        for (int kt = 0; kt < KT; ++kt) {
+            uint4 k[CH];
+            keys(kt, k);
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                const bool check = 64 * (c + 1) > 32 * S::LEAST * static_cast<int>(sizeof(T));
-                if (check && 64 * c + 16 * G >= row_bytes) t.k[kt][c] = make_uint4(0, 0, 0, 0);
-            }
-        float p[RT][4 * KT];
+            for (int c = 0; c < CH; ++c)
+                if (maybe_behind(c) && 64 * c + 16 * G >= row_bytes) k[c] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
+            for (int rt = 0; rt < RT; ++rt) {
                 f32x4 s{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
                     if constexpr (sizeof(T) == 2) {
-                        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t.k[kt][c]), __builtin_bit_cast(bf16x8, q[rt][c]), s, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[c]), __builtin_bit_cast(bf16x8, q[rt][c]), s, 0, 0, 0);
                     } else {
-                        const f32x4 kf = __builtin_bit_cast(f32x4, t.k[kt][c]), qf = __builtin_bit_cast(f32x4, q[rt][c]);
+                        const f32x4 kf = __builtin_bit_cast(f32x4, k[c]), qf = __builtin_bit_cast(f32x4, q[rt][c]);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[i], qf[i], s, 0, 0, 0);
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p[rt][4 * kt + i] = s[i] * a.scale_log2e;
-            }
-        bool special = false;
-        if (!all_seen) {
-            unsigned mine = 0, odd = 0;       // which of the lane's keys exist; whether one of them holds what is not finite
-#pragma unroll
-            for (int j = 0; j < 4 * KT; ++j) {
-                const unsigned there = t.valid >> (16 * (j / 4) + 4 * G + j % 4) & 1;
-                mine |= there << j;
-#pragma unroll
-                for (int w = 0; w < CH; ++w) {
-                    t.v[j][w] &= 0u - there;
-                    odd |= not_finite(t.v[j][w], T{});
-                }
-            }
-            special = __any(odd != 0);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                unsigned seen = mine;
-                if (of_nodes) {
-                    const unsigned bits = static_cast<unsigned>(a.ancestors[static_cast<size_t>(token[rt]) * a.words + at0 / 64] >> (at0 % 64)) >> (4 * G);
-                    seen &= (bits & 15u) | (KT == 2 ? (bits >> 16 & 15u) << 4 : 0u);
-                }
-                if (a.window > 0)
-#pragma unroll
-                    for (int j = 0; j < 4 * KT; ++j) {
-                        const int k = at0 + 16 * (j / 4) + 4 * G + j % 4;
-                        const int at = of_nodes ? a.positions[first + min(k, nodes - 1)] : k;
-                        seen &= ~((at < low[rt] ? 1u : 0u) << j);
-                    }
-#pragma unroll
-                for (int j = 0; j < 4 * KT; ++j) p[rt][j] = seen >> j & 1 ? p[rt][j] : -INFINITY;
+                for (int i = 0; i < 4; ++i) p[rt][4 * kt + i] = s[i] * scale_log2e;
             }
         }
+    }
+    // Scores to weights. The maximum that weights are taken against follows only when one lies 8 above it: weights then reach 2^8, which costs
+    // no accuracy, and most tiles leave sums and outputs as they are.
+    __device__ __forceinline__ void weights(float (&p)[RT][4 * KT]) {
+        float fix[RT];
+        bool any = false;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             float mx = p[rt][0];
 #pragma unroll
             for (int j = 1; j < 4 * KT; ++j) mx = fmaxf(mx, p[rt][j]);
             mx = rows_max(mx);
-            // The maximum that weights are taken against follows only when one lies 8 above it: weights then reach 2^8, which costs no
-            // accuracy, and most tiles leave sum and outputs as they are.
             const bool more = mx > m[rt] + 8.f;
-            if (__any(more)) {
-                const float fix = more ? exp2_for<T>(m[rt] - mx) : 1.f;
-                m[rt] = more ? mx : m[rt];
-                ref[rt] = more ? mx : ref[rt];
-                l[rt] *= fix;
+            fix[rt] = more ? exp2_for<T>(m[rt] - mx) : 1.f;
+            m[rt] = more ? mx : m[rt];
+            ref[rt] = more ? mx : ref[rt];
+            any = any || more;
+        }
+        if (__any(any))
 #pragma unroll
-                for (int x = 0; x < TILES; ++x)
+            for (int rt = 0; rt < RT; ++rt) {
+                l[rt] *= fix[rt];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[x][rt][i] *= fix;
+                for (int x = 0; x < TILES; ++x) o[x][rt] *= fix[rt];
             }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
             float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < 4 * KT; ++j) {
@@ -354,89 +247,351 @@ __global__ void __launch_bounds__(MAXW * 64) tree_attention_kernel(TreeAttention
             }
             l[rt] += sum;
         }
-        auto add = [&](int x, int rt, auto&& product) { o[x][rt] = product(o[x][rt]); };
-        if (!special) {
-            weigh(t.v, p, std::false_type{}, 0, add);
-            return;
+    }
+
+    // A tile whose keys all rows see.
+    template <typename K, typename V>
+    __device__ __forceinline__ void take(float scale_log2e, int row_bytes, K&& keys, V&& values) {
+        float p[RT][4 * KT];
+        scores(p, scale_log2e, row_bytes, keys);
+        uint32_t v[4 * KT][CH];
+        values(v);
+        weights(p);
+        weigh<false>([&](int j, int w) { return v[j][w]; }, [&](int rt, int j) { return p[rt][j]; },
+                     [&](int x, int rt, auto&& product) { o[x][rt] = product(o[x][rt]); });
+    }
+    // Any tile: keys [at0, at0 + KEYS) of the cache, or of the nodes; `valid` has a bit for each that exists. stored(j, w) gives a word of the values.
+    template <typename K, typename W>
+    __device__ __forceinline__ void take_some(const TreeAttentionParams& a, bool of_nodes, int at0, unsigned valid, int first, int nodes, int row_bytes, K&& keys, W&& stored) {
+        const int G = threadIdx.x % 64 / 16;
+        float p[RT][4 * KT];
+        scores(p, a.scale_log2e, row_bytes, keys);
+        unsigned mine = 0;                   // which of the lane's keys exist
+#pragma unroll
+        for (int j = 0; j < 4 * KT; ++j) mine |= (valid >> (16 * (j / 4) + 4 * G + j % 4) & 1) << j;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            unsigned seen = mine;
+            if (of_nodes) {
+                const unsigned bits = static_cast<unsigned>(a.ancestors[static_cast<size_t>(token[rt]) * a.words + at0 / 64] >> (at0 % 64)) >> (4 * G);
+                seen &= (bits & 15u) | (KT == 2 ? (bits >> 16 & 15u) << 4 : 0u);
+            }
+            if (a.window > 0)
+#pragma unroll
+                for (int j = 0; j < 4 * KT; ++j) {
+                    const int k = at0 + 16 * (j / 4) + 4 * G + j % 4;
+                    const int at = of_nodes ? a.positions[first + min(k, nodes - 1)] : k;
+                    seen &= ~((at < low[rt] ? 1u : 0u) << j);
+                }
+#pragma unroll
+            for (int j = 0; j < 4 * KT; ++j) p[rt][j] = seen >> j & 1 ? p[rt][j] : -INFINITY;
         }
-        // A tile of which some rows see less than others holds a value that is not finite: zero times it would reach those that do not see
-        // it. The finite values are weighed as ever; whether a row gives weight to a NaN, +inf or -inf of a column is a product of ones and zeros.
-        weigh(t.v, p, std::true_type{}, 0, add);
+        weights(p);
+        // A key that does not exist has some other row's values. A value that is not finite, in a tile of which some rows see less than others,
+        // would reach those that do not see it as zero times it: the finite values are weighed as ever, and whether a row gives weight to a NaN,
+        // +inf or -inf of a column is a product of ones and zeros. (The words are read anew for each, which keeps them out of the registers.)
+        auto word = [&](int j, int w) { return stored(j, w) & (0u - (mine >> j & 1)); };
+        auto weight = [&](int rt, int j) { return p[rt][j]; };
+        auto add = [&](int x, int rt, auto&& product) { o[x][rt] = product(o[x][rt]); };
+        uint32_t odd = 0;
+#pragma unroll
+        for (int w = 0; w < CH; ++w) {
+#pragma unroll
+            for (int j = 0; j < 4 * KT; ++j) odd |= not_finite(word(j, w), T{});
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        asm volatile("" ::: "memory");
+        const bool special = __any(odd != 0);
+        weigh<true>([&](int j, int w) { return special ? sifted(word(j, w), 0, T{}) : word(j, w); }, weight, add);
+        if (!special) return;
 #pragma unroll 1
         for (int kind = 1; kind <= 3; ++kind) {
             const float value = kind == 1 ? __builtin_nanf("") : kind == 2 ? INFINITY : -INFINITY;
-            weigh(t.v, p, std::true_type{}, kind, [&](int x, int rt, auto&& product) {
-                const f32x4 count = product(f32x4{0.f, 0.f, 0.f, 0.f});
+            asm volatile("" ::: "memory");
+            weigh<true>([&](int j, int w) { return sifted(word(j, w), kind, T{}); }, [&](int rt, int j) { return p[rt][j] == 0.f ? 0.f : 1.f; },
+                        [&](int x, int rt, auto&& product) {
+                            const f32x4 count = product(f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[x][rt][i] += count[i] > 0.f ? value : 0.f;
-            });
+                            for (int i = 0; i < 4; ++i) o[x][rt][i] += count[i] > 0.f ? value : 0.f;
+                        });
+        }
+    }
+
+    // Where o[x][rt][i] stands in its row: column() + E(x) * (4 G + i), E elements a lane has in the block.
+    __device__ __forceinline__ static constexpr int each(int x) { return S::block_words(x / S::PER) * S::PER; }
+    __device__ __forceinline__ static constexpr int column(int x) {
+        return S::block_first(x / S::PER) * 16 * S::PER + (x / S::PER - S::block_first(x / S::PER)) * S::PER + x % S::PER;
+    }
+};
+
+// What a workgroup works on, the same in all its threads.
+struct Work {
+    int b, hk, split, row_tile, group, first, nodes, rows, cached;
+    // Workgroups that share keys have numbers 8 apart, so that they run on one XCD and the second finds the keys in its L2.
+    __device__ __forceinline__ bool find(const TreeAttentionParams& a, int rows_each) {
+        const int residue = blockIdx.x % 8, rest = blockIdx.x / 8;
+        const int unit = rest / a.row_tiles * 8 + residue;
+        row_tile = rest % a.row_tiles;
+        if (unit >= a.units) return false;
+        split = unit % a.nsplit;
+        hk = unit / a.nsplit % a.n_kv_heads;
+        b = unit / a.nsplit / a.n_kv_heads;
+        group = a.n_heads / a.n_kv_heads;
+        first = min(max(a.cu_q[b], 0), a.tokens);
+        nodes = min(min(max(a.cu_q[b + 1] - first, 0), a.tokens - first), a.max_new);
+        rows = nodes * group;
+        cached = static_cast<int>(min(min(static_cast<long long>(max(a.cached[b], 0)), static_cast<long long>(a.max_blocks) * a.page_size), INT32_MAX - 128ll));
+        return row_tile * rows_each < rows;
+    }
+};
+
+__device__ __forceinline__ int block_of(const TreeAttentionParams& a, int at) {
+    return static_cast<int>((static_cast<unsigned long long>(static_cast<unsigned>(at)) * a.page_magic) >> a.page_shift);
+}
+__device__ __forceinline__ float2* split_state(const TreeAttentionParams& a, size_t pair) {
+    return reinterpret_cast<float2*>(a.ws + static_cast<size_t>(a.tokens) * a.n_heads * a.nsplit * a.head_dim) + pair;
+}
+
+// 16-byte piece p of row k of a stage lies at piece p ^ k (rotated by k where a row's pieces are no power of two), so that 16 lanes that
+// read one piece of 16 rows meet no bank twice.
+constexpr int TABLE_ENTRIES = 2048;
+template <typename T, int NT, int NW, int KG>
+struct Stage {
+    using S = Shape<T, NT>;
+    static constexpr int ROW = S::CH * 64, PIECES = 4 * S::CH, LEAST = S::KEYS * KG;      // a key group has one tile of a stage at least
+    static constexpr int keys() {          // 16 KB of keys and values at least, in whole instructions of all wavefronts
+        int n = LEAST;
+        while (n * 2 * ROW < 16384 || n * PIECES % (64 * NW) != 0) n *= 2;
+        return n;
+    }
+    static constexpr int KEYS = keys();
+    static constexpr int MATRIX = KEYS * ROW, BYTES = 2 * MATRIX;
+    static constexpr int NUMBER = 5 * BYTES <= 81920 ? 5 : 4 * BYTES <= 81920 ? 4 : 3 * BYTES <= 131072 ? 3 : 2;
+    static constexpr int LOADS = KEYS * PIECES / 64 / NW;                 // of a wavefront, a stage and matrix
+    static_assert(LOADS * 64 * NW == KEYS * PIECES, "whole instructions");
+    static constexpr int WORDS = (KEYS + 63) / 64;
+};
+
+template <typename T, int NT, int RT, int NW, int KG>
+__global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionParams a) {
+    using R = Rows<T, NT, RT>;
+    using S = Shape<T, NT>;
+    using St = Stage<T, NT, NW, KG>;
+    constexpr int KT = S::KT, KEYS = S::KEYS, CH = S::CH, TILES = S::TILES, PIECES = St::PIECES, SK = St::KEYS, RG = NW / KG, PITCH = 32 * NT + 4;
+    constexpr bool POW2 = (PIECES & (PIECES - 1)) == 0;
+    // the stages [keys, values][SK][PIECES * 16]; at the end the states [wavefront][16 RT][PITCH], then their maxima and sums
+    extern __shared__ __attribute__((aligned(16))) unsigned char stage_s[];
+    __shared__ int table_s[TABLE_ENTRIES];
+    __shared__ unsigned long long valid_s[St::NUMBER][St::WORDS];         // a bit a key that exists
+    Work w;
+    if (!w.find(a, 16 * RT * RG)) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int kg = wave % KG, rg = wave / KG, group0 = w.row_tile * RG * 16 * RT, row0 = group0 + rg * 16 * RT;
+    const int G = lane / 16, c16 = lane % 16, row_bytes = a.head_dim * static_cast<int>(sizeof(T));
+    const int first = w.first, nodes = w.nodes, hk = w.hk, cached = w.cached;
+    const int* table = a.block_tables + static_cast<size_t>(w.b) * a.max_blocks;
+
+    // A part of the block table lies in LDS, from entry `base` on; all of the workgroup meet here.
+    int base = 0, filled = 0;
+    auto fill_table = [&](int from) {
+        lds_barrier();
+        base = from;
+        filled = min(TABLE_ENTRIES, a.max_blocks - from);
+        for (int i = threadIdx.x; i < filled; i += NW * 64) table_s[i] = table[from + i];
+        __syncthreads();
+    };
+    // Tiles of SK keys: those of the cache from the window's first on, then the nodes'. A split has `per` neighbouring ones.
+    int first_tile = 0;
+    if (a.window > 0) {        // the least position of the workgroup's rows
+        int least = INT32_MAX;
+        const int last = min(group0 + 16 * RT * RG, w.rows) - 1;
+        for (int node = group0 / w.group + static_cast<int>(threadIdx.x); node <= last / w.group; node += NW * 64) least = min(least, a.positions[first + node]);
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) least = min(least, __shfl_xor(least, off, 64));
+        if (lane == 0) table_s[wave] = least;
+        __syncthreads();
+        for (int i = 0; i < NW; ++i) least = min(least, table_s[i]);
+        first_tile = __builtin_amdgcn_readfirstlane(min(max(least - a.window + 1, 0), cached) / SK);
+    }
+    const int cache_tiles = (cached + SK - 1) / SK - first_tile, all_tiles = cache_tiles + (nodes + SK - 1) / SK;
+    const int per = (all_tiles + a.nsplit - 1) / a.nsplit, begin = w.split * per, end = min(all_tiles, begin + per);
+    // The queries come with the table, and are waited for here: a load that the compiler knows of and has not waited for in front of the loop
+    // would have it wait in the loop, every time, for all that is on its way.
+    R r;
+    r.begin(a, first, w.rows, w.group, hk, row0, row_bytes);
+    if (begin < cache_tiles) fill_table(min(block_of(a, (begin + first_tile) * SK), a.max_blocks - 1));
+    r.wait_for_queries(row_bytes);
+
+    const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)stage_s));
+    const size_t head = static_cast<size_t>(hk) * row_bytes;
+    // Asks for a stage. (All of the workgroup come here, behind a barrier after which nobody reads what it fills.)
+    auto ask = [&](int tile) {
+        const bool of_nodes = tile >= cache_tiles;
+        const int at0 = (of_nodes ? tile - cache_tiles : tile + first_tile) * SK, place = tile % St::NUMBER;
+        int lane = threadIdx.x % 64;
+        asm volatile("" : "+v"(lane));         // (what follows from it is worked out here, not kept in registers over the whole loop)
+        if (!of_nodes && block_of(a, min(at0 + SK, cached) - 1) >= base + filled) fill_table(block_of(a, at0));
+        auto row_of = [&](int k, bool& there) {
+            if (of_nodes) {
+                there = at0 + k < nodes;
+                return first + min(at0 + k, nodes - 1);
+            }
+            const int at = min(at0 + k, cached - 1), block = block_of(a, at), entry = table_s[block - base];
+            there = at0 + k < cached && static_cast<unsigned>(entry) < static_cast<unsigned>(a.n_pages);
+            return there ? entry * a.page_size + at - block * a.page_size : 0;
+        };
+#pragma unroll
+        for (int i = 0; i < St::WORDS; ++i)
+            if (i % NW == wave) {
+                bool there;
+                row_of(64 * i + lane % SK, there);
+                const unsigned long long bits = __ballot(there && lane < SK);
+                if (lane == 0) valid_s[place][i] = bits;
+            }
+        const unsigned to = lds0 + place * St::BYTES + wave * St::LOADS * 1024;
+        const unsigned char* kb = reinterpret_cast<const unsigned char*>(of_nodes ? a.k : a.k_pages) + head;
+        const unsigned char* vb = reinterpret_cast<const unsigned char*>(of_nodes ? a.v : a.v_pages) + head;
+        const size_t k_pitch = of_nodes ? a.ldk : a.page_pitch, v_pitch = of_nodes ? a.ldv : a.page_pitch;
+#pragma unroll
+        for (int i = 0; i < St::LOADS; ++i) {
+            const int slot = (wave * St::LOADS + i) * 64 + lane, k = slot / PIECES, there = slot % PIECES;
+            const int piece = POW2 ? there ^ (k & (PIECES - 1)) : (there + PIECES - k % PIECES) % PIECES;
+            const int off = 16 * piece < row_bytes ? 16 * piece : 0;
+            bool ignored;
+            const size_t row = row_of(k, ignored);
+            load_to_lds(kb, row * k_pitch + off, to + 1024 * i);
+            load_to_lds(vb, row * v_pitch + off, to + St::MATRIX + 1024 * i);
         }
     };
+    auto place_of = [&](int k, int piece) { return 16 * (POW2 ? piece ^ (k & (PIECES - 1)) : (piece + k) % PIECES); };
 
-    // One tile is multiplied while the wavefront's next is on its way and the page of the one after it is asked for.
-    {
-        Tile t0, t1;
-        int tile = begin + wave, entry = 0, entry1 = 0;
-        if (tile < end) {
-            entry = ask_entry(tile);
-            entry1 = ask_entry(tile + n_waves);
-            ask(tile, entry, t0);
+    for (int i = 0; i < St::NUMBER - 1; ++i)
+        if (begin + i < end) ask(begin + i);
+    // One loop over the wavefront's tiles of all stages: in two loops, one in the other, the outputs would be copied from the one's registers
+    // to the other's for every tile. (A wavefront whose rows lie behind the last works on the last again, and writes nothing.)
+    constexpr int TURNS = SK / KEYS / KG;
+    bool all_seen = false;
+    for (int step = 0; step < (end - begin) * TURNS; ++step) {
+        const int turn = step % TURNS, tile = begin + step / TURNS;
+        const bool of_nodes = tile >= cache_tiles;
+        const int at0 = (of_nodes ? tile - cache_tiles : tile + first_tile) * SK, place = tile % St::NUMBER;
+        if (turn == 0) {
+            // this stage has come (those behind it may be on their way), and all have read the one before it
+            wait_tiles_and_meet<St::NUMBER - 2, 2 * St::LOADS>(min(St::NUMBER - 2, end - 1 - tile));
+            if (tile + St::NUMBER - 1 < end) ask(tile + St::NUMBER - 1);
+            unsigned long long whole = ~0ull;
+#pragma unroll
+            for (int i = 0; i < St::WORDS; ++i) whole &= valid_s[place][i];
+            if (SK < 64) whole |= ~0ull << (SK % 64);
+            all_seen = !of_nodes && (a.window <= 0 || at0 >= r.low_most) && __builtin_amdgcn_readfirstlane(whole == ~0ull);
         }
-        while (tile < end) {
-            const int next = tile + n_waves;
-            entry = ask_entry(next + n_waves);
-            if (next < end) ask(next, entry1, t1);
-            take(tile, t0);
-            if (next >= end) break;
-            const int after = next + n_waves;
-            entry1 = ask_entry(after + n_waves);
-            if (after < end) ask(after, entry, t0);
-            take(next, t1);
-            tile = after;
+        const unsigned char* keys = stage_s + place * St::BYTES;
+        const int k0 = (turn * KG + kg) * KEYS;
+        auto keys_of = [&](int kt, uint4 (&k)[CH]) {
+            const int row = k0 + 16 * kt + c16;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) k[c] = *reinterpret_cast<const uint4*>(keys + row * St::ROW + place_of(row, 4 * c + G));
+        };
+        if (all_seen) {
+            r.take(a.scale_log2e, row_bytes, keys_of, [&](uint32_t (&v)[4 * KT][CH]) {
+#pragma unroll
+                for (int j = 0; j < 4 * KT; ++j) {
+                    const int row = k0 + 16 * (j / 4) + 4 * G + j % 4;
+                    const unsigned char* at = keys + St::MATRIX + row * St::ROW;
+#pragma unroll
+                    for (int x = 0; x < CH; x += S::block_words(x)) {
+                        if (S::block_words(x) == 4) {
+                            const uint4 u = *reinterpret_cast<const uint4*>(at + place_of(row, 4 * x + c16));
+                            v[j][x] = u.x; v[j][x + 1] = u.y; v[j][x + 2] = u.z; v[j][x + 3] = u.w;
+                        } else if (S::block_words(x) == 2) {
+                            const uint2 u = *reinterpret_cast<const uint2*>(at + place_of(row, 4 * x + c16 / 2) + 8 * (c16 % 2));
+                            v[j][x] = u.x; v[j][x + 1] = u.y;
+                        } else {
+                            v[j][x] = *reinterpret_cast<const uint32_t*>(at + place_of(row, 4 * x + c16 / 4) + 4 * (c16 % 4));
+                        }
+                    }
+                }
+            });
+        } else {
+            const unsigned some = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(valid_s[place][k0 / 64] >> (k0 % 64))) & R::ALL;
+            r.take_some(a, of_nodes, at0 + k0, some, first, nodes, row_bytes, keys_of, [&](int j, int x) {
+                const int row = k0 + 16 * (j / 4) + 4 * G + j % 4, n = S::block_words(x), byte = 64 * S::block_first(x) + 4 * n * c16 + 4 * (x % n);
+                return *reinterpret_cast<const uint32_t*>(keys + St::MATRIX + row * St::ROW + place_of(row, byte / 16) + byte % 16);
+            });
         }
     }
 
-    // The wavefronts' states meet in LDS; every thread merges some rows' columns in the wavefronts' order.
-    float2* ml_s = reinterpret_cast<float2*>(state_s + n_waves * 16 * RT * PITCH);
+    if constexpr (KG == 1) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int row = row0 + 16 * rt + c16;
+            const float sum = rows_sum(r.l[rt]);
+            if (row >= w.rows) continue;
+            const int node = row / w.group, t = first + node, h = hk * w.group + row - node * w.group;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            T* to = reinterpret_cast<T*>(a.out + t * a.ldo) + h * a.head_dim;
+            const size_t pair = (static_cast<size_t>(t) * a.n_heads + h) * a.nsplit + w.split;
+            float* part = a.ws + pair * a.head_dim;
+#pragma unroll
+            for (int x = 0; x < TILES; x += R::each(x))
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int d = R::column(x) + R::each(x) * (4 * G + i);
+                    if (d >= a.head_dim) continue;
+#pragma unroll
+                    for (int e = 0; e < R::each(x); ++e) {
+                        if (a.nsplit == 1) to[d + e] = from_float<T>(r.o[x + e][rt][i] * inv);
+                        else part[d + e] = r.o[x + e][rt][i];
+                    }
+                }
+            if (a.nsplit > 1 && G == 0) *split_state(a, pair) = make_float2(r.m[rt], sum);
+        }
+        return;
+    }
+    // The key groups' states meet in LDS; every thread merges some rows' columns in the groups' order.
+    lds_barrier();              // (the last stage has been read; no load is on its way)
+    float* state_s = reinterpret_cast<float*>(stage_s);
+    float2* ml_s = reinterpret_cast<float2*>(state_s + NW * 16 * RT * PITCH);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const float sum = rows_sum(l[rt]);
-        if (G == 0) ml_s[wave * 16 * RT + 16 * rt + c16] = make_float2(m[rt], sum);
+        const float sum = rows_sum(r.l[rt]);
+        if (G == 0) ml_s[wave * 16 * RT + 16 * rt + c16] = make_float2(r.m[rt], sum);
         float* to = state_s + (wave * 16 * RT + 16 * rt + c16) * PITCH;
 #pragma unroll
-        for (int x = 0; x < TILES; ++x) {
-            const int w = x / S::PER, E = S::block_words(w) * S::PER, base = S::block_first(w) * 16 * S::PER, e = (w - S::block_first(w)) * S::PER + x % S::PER;
+        for (int x = 0; x < TILES; ++x)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) to[base + E * (4 * G + i) + e] = o[x][rt][i];
-        }
+            for (int i = 0; i < 4; ++i) to[R::column(x) + R::each(x) * (4 * G + i)] = r.o[x][rt][i];
     }
-    __syncthreads();
-    const int quads = a.head_dim / 4, count = min(16 * RT, rows - row0);
-    for (int item = threadIdx.x; item < count * quads; item += blockDim.x) {
-        const int r = item / quads, d = (item - r * quads) * 4;
+    lds_barrier();
+    const int quads = a.head_dim / 4, count = min(16 * RT * RG, w.rows - group0);
+    for (int item = threadIdx.x; item < count * quads; item += NW * 64) {
+        const int row = item / quads, d = (item - row * quads) * 4;
+        const int at = row / (16 * RT) * KG * 16 * RT + row % (16 * RT);        // in the first key group's state; the others' lie 16 RT rows apart
         float top = -INFINITY, sum = 0.f;
-        for (int w = 0; w < n_waves; ++w) top = fmaxf(top, ml_s[w * 16 * RT + r].x);
+#pragma unroll
+        for (int i = 0; i < KG; ++i) top = fmaxf(top, ml_s[at + i * 16 * RT].x);
         const float against = top == -INFINITY ? 0.f : top;
         f32x4 v{0.f, 0.f, 0.f, 0.f};
-        for (int w = 0; w < n_waves; ++w) {
-            const float2 ml = ml_s[w * 16 * RT + r];
-            const f32x4 part = *reinterpret_cast<const f32x4*>(state_s + (w * 16 * RT + r) * PITCH + d);
+#pragma unroll
+        for (int i = 0; i < KG; ++i) {
+            const float2 ml = ml_s[at + i * 16 * RT];
+            const f32x4 part = *reinterpret_cast<const f32x4*>(state_s + (at + i * 16 * RT) * PITCH + d);
             const float weight = exp2_for<T>(ml.x - against);
-            if (ml.y == 0.f) continue;          // (a wavefront whose keys nobody saw)
+            if (ml.y == 0.f) continue;          // (a key group whose keys nobody saw)
             sum += weight * ml.y;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += weight * part[i];
+            for (int e = 0; e < 4; ++e) v[e] += weight * part[e];
         }
-        const int node = (row0 + r) / group, t = first + node, h = hk * group + row0 + r - node * group;
+        const int node = (group0 + row) / w.group, t = first + node, h = hk * w.group + group0 + row - node * w.group;
         if (a.nsplit == 1) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             T* to = reinterpret_cast<T*>(a.out + t * a.ldo) + h * a.head_dim + d;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) to[i] = from_float<T>(v[i] * inv);
+            for (int e = 0; e < 4; ++e) to[e] = from_float<T>(v[e] * inv);
         } else {
-            const size_t pair = (static_cast<size_t>(t) * a.n_heads + h) * a.nsplit + split;
+            const size_t pair = (static_cast<size_t>(t) * a.n_heads + h) * a.nsplit + w.split;
             *reinterpret_cast<f32x4*>(a.ws + pair * a.head_dim + d) = v;
-            if (d == 0) *reinterpret_cast<float2*>(a.ws + static_cast<size_t>(a.tokens) * a.n_heads * a.nsplit * a.head_dim + 2 * pair) = make_float2(top, sum);
+            if (d == 0) *split_state(a, pair) = make_float2(top, sum);
         }
     }
 }
@@ -472,52 +627,61 @@ __global__ void __launch_bounds__(256) tree_attention_join_kernel(TreeAttentionP
     }
 }
 
-// How a call is shared out: rows of a workgroup, wavefronts, workgroups that share a row's keys.
+// How a call is shared out: 16-row tiles of a wavefront, wavefronts of a workgroup, key groups among them, workgroups that share a row's keys.
 struct Plan {
-    int nt, rt, waves, row_tiles, nsplit;
+    int nt, rt, waves, key_groups, row_tiles, nsplit;
 };
 
 Plan plan_of(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_new, int max_cached, int window, int dtype) {
     Plan p;
+    const bool f32 = dtype == MLLM_F32;
     p.nt = (head_dim + 31) / 32;
     if (p.nt == 5) p.nt = 6;
     if (p.nt == 7) p.nt = 8;
     const long long rows = static_cast<long long>(max_new) * (n_heads / n_kv_heads);
-    p.rt = rows <= 16 ? 1 : rows <= 32 || p.nt > 4 || (dtype == MLLM_F32 && p.nt > 2) ? 2 : 4;
-    if (dtype == MLLM_F32 && p.nt > 4) p.rt = 1;
-    p.waves = p.rt == 4 || p.nt >= 4 || p.nt * p.rt >= 6 || (dtype == MLLM_F32 && p.nt > 2) ? 4 : 8;
-    p.row_tiles = static_cast<int>((rows + 16 * p.rt - 1) / (16 * p.rt));
-    const int keys = dtype == MLLM_F32 ? 16 : 32;
+    const int most = p.nt <= 2 ? 8 : p.nt <= 4 ? 4 : 2;          // key groups whose stage fits twice
+    p.rt = 1;
+    int row_groups = 1;
+    if (rows > 16) row_groups = 2;
+    if (rows > 32) row_groups = 4;
+    if (rows > 64) { row_groups = p.nt <= 4 ? 4 : 8; p.rt = p.nt <= 4 ? 2 : 1; }
+    if (rows > 128 && p.nt <= 4) row_groups = 8;
+    p.waves = p.nt <= 2 ? 8 : std::min(8, row_groups * most);
+    p.key_groups = p.waves / row_groups;
+    const int each = 16 * p.rt * row_groups;
+    p.row_tiles = static_cast<int>((rows + each - 1) / each);
+    const int keys = f32 ? 16 : 32;
     const long long seen = window > 0 ? std::min<long long>(max_cached, static_cast<long long>(window) + max_new) : max_cached;
     const long long tiles = (seen + keys - 1) / keys + (max_new + keys - 1) / keys;
     const long long groups = static_cast<long long>(n_seqs) * n_kv_heads * p.row_tiles;
-    p.nsplit = static_cast<int>(std::max<long long>(1, std::min<long long>({512 / groups, tiles / (4 * p.waves), 64})));
+    p.nsplit = static_cast<int>(std::max<long long>(1, std::min<long long>({512 / groups, tiles / (4 * p.key_groups), 64})));
     return p;
 }
 
-template <typename T, int NT, int RT, int MAXW>
-int launch(const TreeAttentionParams& p, int waves, hipStream_t stream) {
-    const size_t lds = static_cast<size_t>(waves) * 16 * RT * ((32 * NT + 4) * 4 + 8);
-    auto kernel = tree_attention_kernel<T, NT, RT, MAXW>;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
-    if (e != hipSuccess) return static_cast<int>(e);
+template <typename T, int NT, int RT, int NW, int KG>
+int launch(const TreeAttentionParams& p, hipStream_t stream) {
+    using St = Stage<T, NT, NW, KG>;
     const long long blocks = (static_cast<long long>(p.units) + 7) / 8 * 8 * p.row_tiles;
     if (blocks > INT32_MAX) return -1;
-    kernel<<<static_cast<unsigned>(blocks), waves * 64, lds, stream>>>(p);
+    constexpr int STATES = KG == 1 ? 0 : NW * 16 * RT * ((32 * NT + 4) * 4 + 8), LDS = std::max(St::NUMBER * St::BYTES, STATES);
+    static_assert(LDS + TABLE_ENTRIES * 4 + 1024 <= 163840, "LDS of a compute unit");
+    auto kernel = tree_attention_kernel<T, NT, RT, NW, KG>;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (e != hipSuccess) return static_cast<int>(e);
+    kernel<<<static_cast<unsigned>(blocks), NW * 64, LDS, stream>>>(p);
     return 0;
 }
 
 template <typename T>
 int dispatch(const TreeAttentionParams& p, const Plan& plan, hipStream_t stream) {
-#define TREE_CASE(N, R, W) if (plan.nt == N && plan.rt == R) return launch<T, N, R, W>(p, plan.waves, stream);
-    if constexpr (sizeof(T) == 2) {
-        TREE_CASE(1, 1, 8) TREE_CASE(1, 2, 8) TREE_CASE(1, 4, 4) TREE_CASE(2, 1, 8) TREE_CASE(2, 2, 8) TREE_CASE(2, 4, 4)
-        TREE_CASE(3, 1, 8) TREE_CASE(3, 2, 4) TREE_CASE(3, 4, 4) TREE_CASE(4, 1, 4) TREE_CASE(4, 2, 4) TREE_CASE(4, 4, 4)
-        TREE_CASE(6, 1, 4) TREE_CASE(6, 2, 4) TREE_CASE(8, 1, 4) TREE_CASE(8, 2, 4)
-    } else {
-        TREE_CASE(1, 1, 8) TREE_CASE(1, 2, 8) TREE_CASE(1, 4, 4) TREE_CASE(2, 1, 8) TREE_CASE(2, 2, 8) TREE_CASE(2, 4, 4)
-        TREE_CASE(3, 1, 4) TREE_CASE(3, 2, 4) TREE_CASE(4, 1, 4) TREE_CASE(4, 2, 4) TREE_CASE(6, 1, 4) TREE_CASE(8, 1, 4)
-    }
+#define TREE_CASE(N, R, W, K) if (plan.nt == N && plan.rt == R && plan.waves == W && plan.key_groups == K) return launch<T, N, R, W, K>(p, stream);
+#define TREE_NARROW(N) TREE_CASE(N, 1, 8, 8) TREE_CASE(N, 1, 8, 4) TREE_CASE(N, 1, 8, 2) TREE_CASE(N, 2, 8, 2) TREE_CASE(N, 2, 8, 1)
+#define TREE_MIDDLE(N) TREE_CASE(N, 1, 4, 4) TREE_CASE(N, 1, 8, 4) TREE_CASE(N, 1, 8, 2) TREE_CASE(N, 2, 8, 2) TREE_CASE(N, 2, 8, 1)
+#define TREE_WIDE(N) TREE_CASE(N, 1, 2, 2) TREE_CASE(N, 1, 4, 2) TREE_CASE(N, 1, 8, 2) TREE_CASE(N, 1, 8, 1)
+    TREE_NARROW(1) TREE_NARROW(2) TREE_MIDDLE(3) TREE_MIDDLE(4) TREE_WIDE(6) TREE_WIDE(8)
+#undef TREE_WIDE
+#undef TREE_MIDDLE
+#undef TREE_NARROW
 #undef TREE_CASE
     return -1;
 }

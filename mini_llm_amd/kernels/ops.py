@@ -9,7 +9,9 @@ loaded, raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -107,11 +109,11 @@ def engine_library():
         "mllm_op_linear_stream_add": (_i, [T2p, T2p, _vp, T2p, T2p, T2p, ctypes.POINTER(TanhNormC), ctypes.POINTER(TanhNormC), _vp]),
         "mllm_op_token_side": (_i, [T2p, T2p, T2p, T2p, _vp, _f, _vp, _vp, _vp, _i, T2p, _i, T2p, ctypes.POINTER(TanhNormC), _vp]),
         "mllm_op_tree_max_nodes": (_i, []),
-        "mllm_op_step_maps": (_i, [ctypes.POINTER(StepMapsC), _vp]),
-        "mllm_op_rotary": (_i, [T2p, _vp, _vp, _i, _i, _i, _i, _f, T2p, _vp]),
-        "mllm_op_tree_attention_workspace": (_i, [ctypes.POINTER(TreeAttentionC), ctypes.POINTER(ctypes.c_ulonglong)]),
-        "mllm_op_tree_attention": (_i, [ctypes.POINTER(TreeAttentionC), _vp]),
-        "mllm_op_tree_accept": (_i, [ctypes.POINTER(TreeAcceptC), _vp]),
+        "mllm_op_step_maps": (_i, [_vp, _vp]),
+        "mllm_op_rotary": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp]),
+        "mllm_op_tree_attention_workspace": (ctypes.c_longlong, [_i] * 9),
+        "mllm_op_tree_attention": (_i, [_vp, _vp]),
+        "mllm_op_tree_accept": (_i, [_vp, _vp]),
         "mllm_op_argmax": (_i, [T2p, _vp, _vp]),
         "mllm_op_sample": (_i, [T2p, _vp, _vp, _vp, _vp]),
     }
@@ -642,23 +644,67 @@ def tree_max_nodes() -> int:
     return int(engine_library().mllm_op_tree_max_nodes())
 
 
-def _here(*tensors: Optional[torch.Tensor]) -> None:
-    """All on one GPU, and that the current one (whose current stream the op is launched on)."""
-    _gpu(*tensors)
-    for t in tensors:
-        if t is not None and t.device.index != torch.cuda.current_device():
-            raise KernelError(f"tensor is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+def _here(*tensors: Optional[torch.Tensor]) -> int:
+    """All on one GPU, and that the current one (whose current stream the op is launched on); its number."""
+    devices = {t.get_device() for t in tensors if t is not None}
+    if len(devices) > 1 or -1 in devices:
+        _gpu(*tensors)
+        raise KernelError(f"tensors are on GPUs {sorted(devices)}")
+    device = devices.pop()
+    if device != torch.cuda.current_device():
+        raise KernelError(f"tensors are on cuda:{device}, the current device is cuda:{torch.cuda.current_device()}")
+    return device
 
 
-def _counted(t: torch.Tensor, name: str, n: int) -> None:
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != 1 or t.numel() != n:
+def _stream_of(device: int) -> int:
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+
+
+def _counted(t: torch.Tensor, name: str, n: int) -> int:
+    """The address of n whole numbers."""
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
         raise KernelError(f"{name} must be contiguous int32 [{n}], got {tuple(t.shape)} {t.dtype}")
+    return t.data_ptr()
+
+
+def _matrix(t: torch.Tensor, name: str) -> tuple:
+    """The numbers of a Tensor2."""
+    if t.dim() == 2:
+        rows, cols = t.shape
+        across, along = t.stride()
+        dtype = _DT.get(t.dtype)
+        if dtype is not None and along == 1 and (rows > 1 or across >= cols):
+            return t.data_ptr(), dtype, rows, cols, across
+    c = t2(t, name)
+    return c.data or 0, c.dtype, c.rows, c.cols, c.stride
+
+
+# The calls' numbers go into the native structures' bytes at once (a field of a ctypes structure costs as much as its number).
+_MATRIX = "Piqqq"
+_MAPS_BYTES = struct.Struct("@PPPPPqiiiiiiiiPPPPPPPP")
+_ACCEPT_BYTES = struct.Struct("@PPPPPPPiiiiiiiPPPPP")
+_ATTENTION_BYTES = struct.Struct("@" + 3 * _MATRIX + "iii" + 2 * _MATRIX + "iPiiPPPiPfiii" + _MATRIX + "PN")
+_ROWS_BYTES = struct.Struct("@" + _MATRIX)
+
+
+def _bytes(form: struct.Struct, *numbers) -> bytes:
+    try:
+        return form.pack(*numbers)
+    except struct.error as e:
+        raise KernelError(f"a number does not fit: {e}") from None
 
 
 def _table(t: torch.Tensor, name: str, rows: Optional[int] = None) -> None:
     if t.dim() != 2 or t.dtype != torch.int32 or t.shape[0] < 1 or t.shape[1] < 1 or (t.shape[1] > 1 and t.stride(1) != 1) or \
             (rows is not None and t.shape[0] != rows):
         raise KernelError(f"{name} must be int32 [{'requests' if rows is None else rows}, blocks] with contiguous rows, got {tuple(t.shape)} {t.dtype}")
+
+
+def _whole_table(t: torch.Tensor, name: str, rows: int) -> tuple:
+    """Address and columns of a contiguous table."""
+    if t.dim() != 2 or t.dtype is not torch.int32 or not t.is_contiguous() or t.shape[0] != rows or t.shape[1] < 1:
+        raise KernelError(f"{name} must be contiguous int32 [{rows}, {'max_new' if name == 'path' else 'max_blocks'}], got {tuple(t.shape)} {t.dtype}")
+    return t.data_ptr(), t.shape[1]
 
 
 class StepMaps:
@@ -673,12 +719,14 @@ class StepMaps:
         if tree and max_new > tree_max_nodes():
             raise KernelError(f"a tree has at most {tree_max_nodes()} nodes, not {max_new}")
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
-        self.max_new = max_new
+        self.n_seqs, self.tokens, self.max_blocks, self.max_new, self.words = n_seqs, tokens, max_blocks, max_new, (max_new + 63) // 64
         zeros = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=device)      # noqa: E731
         self.cu_q, self.cached, self.ctx_len = zeros(n_seqs + 1), zeros(n_seqs), zeros(n_seqs)
         self.token_seq, self.positions, self.slots = zeros(tokens), zeros(tokens), zeros(tokens)
         self.block_tables = zeros(n_seqs, max_blocks)
-        self.ancestors = torch.zeros((tokens, (max_new + 63) // 64), dtype=torch.int64, device=device) if tree else None
+        self.ancestors = torch.zeros((tokens, self.words), dtype=torch.int64, device=device) if tree else None
+        self.addresses = tuple(0 if t is None else t.data_ptr() for t in (self.cu_q, self.cached, self.ctx_len, self.token_seq, self.positions, self.slots,
+                                                                          self.block_tables, self.ancestors))
 
 
 def step_maps(maps: StepMaps, rows: Optional[torch.Tensor], n_new: torch.Tensor, lengths: torch.Tensor, pages: torch.Tensor, page_size: int,
@@ -693,26 +741,23 @@ def step_maps(maps: StepMaps, rows: Optional[torch.Tensor], n_new: torch.Tensor,
     child counts as none. More than ``max_new`` tokens of a sequence, or more than ``tokens`` together, are left out (cu_q says how
     many are in). A position beyond ``max_blocks``, or whose page is none of the ``n_pages``, has slot -1. Tokens behind the last sequence get
     sequence 0, position 0, slot -1 and no ancestors."""
-    B, T, blocks = maps.cached.numel(), maps.token_seq.numel(), maps.block_tables.shape[1]
-    _counted(n_new, "n_new", B)
+    B, T, blocks, mine = maps.n_seqs, maps.tokens, maps.max_blocks, maps.addresses
+    at_new, at_rows, at_parents, words = _counted(n_new, "n_new", B), 0, 0, 0
     if rows is not None:
-        _counted(rows, "rows", B)
+        at_rows = _counted(rows, "rows", B)
     _table(pages, "pages")
-    if pages.shape[1] < blocks:
-        raise KernelError(f"pages has {pages.shape[1]} blocks a request, the maps {blocks}")
-    _counted(lengths, "lengths", pages.shape[0])
+    requests, cols = pages.shape
+    if cols < blocks:
+        raise KernelError(f"pages has {cols} blocks a request, the maps {blocks}")
+    at_lengths = _counted(lengths, "lengths", requests)
     if parents is not None:
         if maps.ancestors is None:
             raise KernelError("parents need step maps made for trees")
-        _counted(parents, "parents", T)
-    _here(rows, n_new, lengths, pages, parents, maps.cu_q)
-    a = StepMapsC(rows=None if rows is None else rows.data_ptr(), n_new=n_new.data_ptr(), lengths=lengths.data_ptr(), pages=pages.data_ptr(),
-                  parents=None if parents is None else parents.data_ptr(), ld_pages=pages.stride(0) if pages.shape[0] > 1 else pages.shape[1], n_seqs=B,
-                  n_requests=pages.shape[0], tokens=T, page_size=int(page_size), n_pages=int(n_pages), max_blocks=blocks, max_new=maps.max_new,
-                  words=0 if parents is None else maps.ancestors.shape[1], cu_q=maps.cu_q.data_ptr(), cached=maps.cached.data_ptr(),
-                  ctx_len=maps.ctx_len.data_ptr(), token_seq=maps.token_seq.data_ptr(), positions=maps.positions.data_ptr(), slots=maps.slots.data_ptr(),
-                  block_tables=maps.block_tables.data_ptr(), ancestors=None if parents is None else maps.ancestors.data_ptr())
-    _ok(engine_library().mllm_op_step_maps(ctypes.byref(a), _stream()))
+        at_parents, words = _counted(parents, "parents", T), maps.words
+    device = _here(rows, n_new, lengths, pages, parents, maps.cu_q)
+    a = _bytes(_MAPS_BYTES, at_rows, at_new, at_lengths, pages.data_ptr(), at_parents, pages.stride(0) if requests > 1 else cols, B, requests, T, page_size,
+               n_pages, blocks, maps.max_new, words, *mine)
+    _ok(engine_library().mllm_op_step_maps(a, _stream_of(device)))
     return maps
 
 
@@ -767,15 +812,15 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, n_head
     positions[t] * freqs[i] (``rotary_freqs``) and multiplied by ``amplitude``; pairs are columns i and i + len(freqs) of a head, or 2i and
     2i + 1 with ``interleaved``; the columns behind them are handed on. ``out`` may be ``x``. positions: int32 [T], in any order; angles
     are exact to 2^-32 of a turn at any of them."""
-    if freqs.dim() != 1 or freqs.dtype != torch.int64 or not freqs.is_contiguous() or freqs.numel() < 1:
+    if freqs.dim() != 1 or freqs.dtype is not torch.int64 or not freqs.is_contiguous() or freqs.numel() < 1:
         raise KernelError("freqs must be contiguous int64 [pairs] (rotary_freqs)")
     if x.dim() != 2 or x.shape != out.shape:
         raise KernelError(f"rotary: x {tuple(x.shape)} and out {tuple(out.shape)} must be [T, n_heads * head_dim]")
-    _counted(positions, "positions", x.shape[0])
-    tx, to = t2(x, "x"), t2(out, "out")
-    _here(x, positions, freqs, out)
-    _ok(engine_library().mllm_op_rotary(ctypes.byref(tx), _p(positions), _p(freqs), freqs.numel(), int(n_heads), int(head_dim), 1 if interleaved else 0,
-                                        float(amplitude), ctypes.byref(to), _stream()))
+    at = _counted(positions, "positions", x.shape[0])
+    mx, mo = _matrix(x, "x"), _matrix(out, "out")
+    device = _here(x, positions, freqs, out)
+    _ok(engine_library().mllm_op_rotary(_ROWS_BYTES.pack(*mx), at, freqs.data_ptr(), freqs.numel(), n_heads, head_dim, 1 if interleaved else 0, amplitude,
+                                        _ROWS_BYTES.pack(*mo), _stream_of(device)))
     return out
 
 
@@ -793,32 +838,38 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, n_heads: i
     (those beyond are not computed); ``max_cached``, the longest cache, decides how the keys are shared out. A node that sees nothing gets zeros;
     rows of no sequence stay as they are; what is not seen counts for nothing, NaN among it; a table's entry that names no page holds nothing."""
     T, B = q.shape[0], cached.numel()
-    if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or not block_tables.is_contiguous() or block_tables.shape[0] != B or block_tables.shape[1] < 1:
-        raise KernelError(f"block_tables must be contiguous int32 [{B}, max_blocks]")
-    _counted(cached, "cached", B)
-    _counted(cu_q, "cu_q", B + 1)
-    if ancestors.dim() != 2 or ancestors.dtype != torch.int64 or not ancestors.is_contiguous() or ancestors.shape[0] != T:
+    at_tables, blocks = _whole_table(block_tables, "block_tables", B)
+    at_cached, at_cu, at_positions = _counted(cached, "cached", B), _counted(cu_q, "cu_q", B + 1), 0
+    if ancestors.dim() != 2 or ancestors.dtype is not torch.int64 or not ancestors.is_contiguous() or ancestors.shape[0] != T:
         raise KernelError(f"ancestors must be contiguous int64 [{T}, words]")
-    if window and positions is None:
-        raise KernelError("tree_attention: positions are needed with a window")
     if positions is not None:
-        _counted(positions, "positions", T)
-    a = TreeAttentionC()
-    a.q, a.k, a.v, a.k_pages, a.v_pages, a.out = (t2(t, n) for t, n in ((q, "q"), (k, "k"), (v, "v"), (k_pages, "k_pages"), (v_pages, "v_pages"), (out, "out")))
-    _here(q, k, v, k_pages, v_pages, block_tables, cached, cu_q, ancestors, positions, out)
-    a.n_heads, a.n_kv_heads, a.head_dim, a.page_size = int(n_heads), int(n_kv_heads), int(head_dim), int(page_size)
-    a.block_tables, a.n_seqs, a.max_blocks = block_tables.data_ptr(), B, block_tables.shape[1]
-    a.cached, a.cu_q, a.ancestors, a.words = cached.data_ptr(), cu_q.data_ptr(), ancestors.data_ptr(), ancestors.shape[1]
-    a.positions = None if positions is None else positions.data_ptr()
-    a.scale, a.window, a.max_new, a.max_cached = float(scale), int(window or 0), int(max_new), int(max_cached)
-    lib, floats = engine_library(), ctypes.c_ulonglong(0)
-    _ok(lib.mllm_op_tree_attention_workspace(ctypes.byref(a), ctypes.byref(floats)))
-    if floats.value:
+        at_positions = _counted(positions, "positions", T)
+    elif window:
+        raise KernelError("tree_attention: positions are needed with a window")
+    mq, mk, mv, mkp, mvp, mo = _matrix(q, "q"), _matrix(k, "k"), _matrix(v, "v"), _matrix(k_pages, "k_pages"), _matrix(v_pages, "v_pages"), _matrix(out, "out")
+    device = _here(q, k, v, k_pages, v_pages, block_tables, cached, cu_q, ancestors, positions, out)
+
+    def numbers(workspace, floats):
+        return _bytes(_ATTENTION_BYTES, *mq, *mk, *mv, n_heads, n_kv_heads, head_dim, *mkp, *mvp, page_size, at_tables, B, blocks, at_cached, at_cu, ancestors.data_ptr(),
+                      ancestors.shape[1], at_positions, scale, window, max_new, max_cached, *mo, workspace, floats)
+
+    lib = engine_library()
+    try:
+        floats = _tree_workspace(T, B, n_heads, n_kv_heads, head_dim, max_new, max_cached, window, mq[1])
+    except ctypes.ArgumentError:
+        raise KernelError("tree_attention: sizes are whole numbers of 32 bits") from None
+    if floats > 0:
         # (of the caller's stream and, in a capture, of the graph's own pool: two graphs share none)
-        ws = torch.empty(floats.value, dtype=torch.float32, device=q.device)
-        a.workspace, a.workspace_floats = ws.data_ptr(), floats.value
-    _ok(lib.mllm_op_tree_attention(ctypes.byref(a), _stream()))
+        ws = torch.empty(floats, dtype=torch.float32, device=q.device)
+        _ok(lib.mllm_op_tree_attention(numbers(ws.data_ptr(), floats), _stream_of(device)))
+    else:
+        _ok(lib.mllm_op_tree_attention(numbers(0, 0), _stream_of(device)))
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _tree_workspace(*sizes) -> int:
+    return int(engine_library().mllm_op_tree_attention_workspace(*sizes))
 
 
 def tree_accept(choices: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor, cu_q: torch.Tensor, cached: torch.Tensor, block_tables: torch.Tensor,
@@ -831,22 +882,17 @@ def tree_accept(choices: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor,
     each node that stands (position cached[b] + its place on the path), -1 for the others and the rows of no sequence: what ``kv_append`` takes.
     With ``lengths`` (int32 [requests]): lengths[rows[b]] = cached[b] + kept[b] (``rows`` None: b). A page that is none of the ``n_pages`` gives slot -1."""
     T, B = choices.numel(), cached.numel()
-    for t, n in ((choices, "choices"), (ids, "ids"), (parents, "parents"), (slots, "slots")):
-        _counted(t, n, T)
-    for t, n in ((cached, "cached"), (kept, "kept"), (next_token, "next_token")):
-        _counted(t, n, B)
-    _counted(cu_q, "cu_q", B + 1)
-    if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or not block_tables.is_contiguous() or block_tables.shape[0] != B or block_tables.shape[1] < 1:
-        raise KernelError(f"block_tables must be contiguous int32 [{B}, max_blocks]")
-    if path.dim() != 2 or path.dtype != torch.int32 or not path.is_contiguous() or path.shape[0] != B or path.shape[1] < 1:
-        raise KernelError(f"path must be contiguous int32 [{B}, max_new]")
+    tokens = [_counted(t, n, T) for t, n in ((choices, "choices"), (ids, "ids"), (parents, "parents"), (slots, "slots"))]
+    at_cached, at_kept, at_next, at_cu = _counted(cached, "cached", B), _counted(kept, "kept", B), _counted(next_token, "next_token", B), _counted(cu_q, "cu_q", B + 1)
+    at_tables, blocks = _whole_table(block_tables, "block_tables", B)
+    at_path, max_new = _whole_table(path, "path", B)
+    at_rows = at_lengths = requests = 0
     if rows is not None:
-        _counted(rows, "rows", B)
+        at_rows = _counted(rows, "rows", B)
     if lengths is not None:
-        _counted(lengths, "lengths", lengths.numel() if rows is not None else B)
-    _here(choices, ids, parents, cu_q, cached, block_tables, kept, path, next_token, slots, lengths, rows)
-    ptr = lambda t: None if t is None else t.data_ptr()      # noqa: E731
-    a = TreeAcceptC(choices=ptr(choices), ids=ptr(ids), parents=ptr(parents), cu_q=ptr(cu_q), cached=ptr(cached), block_tables=ptr(block_tables), rows=ptr(rows),
-                    n_seqs=B, tokens=T, page_size=int(page_size), n_pages=int(n_pages), max_blocks=block_tables.shape[1], max_new=path.shape[1],
-                    n_requests=0 if lengths is None else lengths.numel(), kept=ptr(kept), path=ptr(path), next=ptr(next_token), slots=ptr(slots), lengths=ptr(lengths))
-    _ok(engine_library().mllm_op_tree_accept(ctypes.byref(a), _stream()))
+        requests = lengths.numel()
+        at_lengths = _counted(lengths, "lengths", requests if rows is not None else B)
+    device = _here(choices, ids, parents, cu_q, cached, block_tables, kept, path, next_token, slots, lengths, rows)
+    a = _bytes(_ACCEPT_BYTES, tokens[0], tokens[1], tokens[2], at_cu, at_cached, at_tables, at_rows, B, T, page_size, n_pages, blocks, max_new, requests, at_kept, at_path,
+               at_next, tokens[3], at_lengths)
+    _ok(engine_library().mllm_op_tree_accept(a, _stream_of(device)))

@@ -35,7 +35,7 @@ def test_tree_attention_refuses(change, match):
 
 
 def native_attention(**change):
-    """A native call whose checks fail (or pass, for the workspace's size) in front of any launch; addresses are never read."""
+    """A native call whose checks fail in front of any launch; addresses are never read."""
     at = lambda i, dt, r, c, s=None: ops.Tensor2(1 << (20 + i), dt, r, c, c if s is None else s)      # noqa: E731
     a = ops.TreeAttentionC()
     dt = change.pop("dtype", 1)
@@ -45,9 +45,7 @@ def native_attention(**change):
     a.block_tables = a.cached = a.cu_q = a.ancestors = a.positions = 1 << 30
     for name, value in change.items():
         setattr(a, name, at(*value) if isinstance(value, tuple) else value)
-    floats = ctypes.c_ulonglong(0)
-    ops._ok(ops.engine_library().mllm_op_tree_attention_workspace(ctypes.byref(a), ctypes.byref(floats)))
-    return floats.value
+    ops._ok(ops.engine_library().mllm_op_tree_attention(ctypes.byref(a), None))
 
 
 @pytest.mark.parametrize("change,match", [
@@ -63,10 +61,25 @@ def test_native_tree_attention_refuses(change, match):
 
 
 def test_native_tree_attention_wants_its_workspace():
-    """What a call says it needs is what it refuses to run without; a cache as long as its numbers go asks for no more than splits of it."""
+    """Few rows of a long cache are split: the call is refused without its workspace. The longest cache that the numbers allow asks for no more
+    than splits of it, and sizes that the call refuses for nothing."""
+    size = ops.engine_library().mllm_op_tree_attention_workspace
     for dtype in (0, 1):
-        need = native_attention(dtype=dtype, max_cached=2 ** 31 - 1)
-        assert need % 1 == 0 and need < 2 ** 32
+        assert 0 < size(3, 2, 4, 2, 16, 3, 2 ** 31 - 1, 0, dtype) < 2 ** 20
+        with pytest.raises(ops.KernelError, match="workspace"):
+            native_attention(dtype=dtype, max_cached=2 ** 31 - 1)
+    assert [size(*s) for s in ((3, 2, 4, 0, 16, 3, 99999, 0, 1), (3, 2, 4, 3, 16, 3, 99999, 0, 1), (3, 2, 4, 2, 300, 3, 99999, 0, 1), (0, 0, 4, 2, 16, 3, 99999, 0, 1))] == [0] * 4
+
+
+def test_structures_are_as_the_native_side_has_them():
+    for form, c in ((ops._MAPS_BYTES, ops.StepMapsC), (ops._ACCEPT_BYTES, ops.TreeAcceptC), (ops._ATTENTION_BYTES, ops.TreeAttentionC), (ops._ROWS_BYTES, ops.Tensor2)):
+        assert form.size == ctypes.sizeof(c)
+
+
+def test_numbers_beyond_32_bits_are_refused():
+    for name in ("max_cached", "page_size", "window"):
+        with pytest.raises(ops.KernelError):
+            ops.tree_attention(**attention_args(**{name: 2 ** 40}))
 
 
 def maps_args(**change):
