@@ -26,6 +26,7 @@
 #include "lds_loads.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace {
@@ -43,15 +44,16 @@ struct TreeAttentionParams {
     unsigned page_magic;                          // at / page_size = (at * page_magic) >> page_shift for 0 <= at < 2^31
     int page_shift;
     int row_tiles, nsplit, units;
-    float scale_log2e;
+    float scale;              // of the products, in base 2, above zero: a negative one is its size, and the queries' sign is turned
+    bool negative;
     char* out;
     float* ws;
 };
 
 // Sizes of a kernel for heads of more than 32 (NT - 1), up to 32 NT columns (less for the NT that stand for two).
-template <typename T, int NT>
+template <typename T, int NT, int KEY_GROUPS_OF_16>
 struct Shape {
-    static constexpr int KT = sizeof(T) == 2 ? 2 : 1;      // 16-key groups of a tile: one product step of values takes 32 keys in bfloat16
+    static constexpr int KT = KEY_GROUPS_OF_16;            // 16-key groups of a tile (bfloat16: a product step of values takes two)
     static constexpr int KEYS = 16 * KT;
     static constexpr int CH = NT * sizeof(T) / 2;          // 64-byte pieces of a row; words of a value row in a lane
     static constexpr int PER = 4 / sizeof(T);              // elements of a word
@@ -68,22 +70,22 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w, float) { return ((w &
 __device__ __forceinline__ uint32_t not_finite(uint32_t w, bf16_t) { return ((w & 0x7f807f80u) + 0x00800080u) >> 15 & 0x00010001u; }
 // kind 0: the elements that are finite, zeros for the others; 1, 2, 3: one where the element is NaN, +inf, -inf, else 0.
 __device__ __forceinline__ uint32_t sifted(uint32_t w, int kind, float) {
-    const uint32_t special = not_finite(w, 0.f), mantissa = (w & 0x7fffffu) + 0x7fffffu >> 23, sign = w >> 31;
+    const uint32_t special = not_finite(w, 0.f), mantissa = ((w & 0x7fffffu) + 0x7fffffu) >> 23, sign = w >> 31;
     if (kind == 0) return w & (special - 1);
     return (special & (kind == 1 ? mantissa : ~mantissa & (kind == 2 ? ~sign : sign))) * 0x3f800000u;
 }
 __device__ __forceinline__ uint32_t sifted(uint32_t w, int kind, bf16_t) {
-    const uint32_t special = not_finite(w, bf16_t{}), mantissa = (w & 0x007f007fu) + 0x007f007fu >> 7, sign = w >> 15;
+    const uint32_t special = not_finite(w, bf16_t{}), mantissa = ((w & 0x007f007fu) + 0x007f007fu) >> 7, sign = w >> 15;
     if (kind == 0) return w & ~(special * 0xffffu);
     return (special & (kind == 1 ? mantissa : ~mantissa & (kind == 2 ? ~sign : sign))) * 0x3f80u;
 }
 
 // One wavefront's rows, 16 RT of them, and what it has summed up for them.
-template <typename T, int NT, int RT>
+template <typename T, int NT, int RT, int KEY_GROUPS_OF_16>
 struct Rows {
-    using S = Shape<T, NT>;
+    using S = Shape<T, NT, KEY_GROUPS_OF_16>;
     static constexpr int KT = S::KT, KEYS = S::KEYS, CH = S::CH, TILES = S::TILES;
-    static constexpr unsigned ALL = KEYS == 32 ? 0xffffffffu : 0xffffu;
+    static constexpr unsigned long long ALL = ~0ull >> (64 - KEYS);
 
     uint4 q[RT][CH];
     f32x4 o[TILES][RT];
@@ -128,12 +130,14 @@ struct Rows {
     }
     // Columns behind the head's last are zero in queries and keys.
     static constexpr bool maybe_behind(int c) { return 64 * (c + 1) > 32 * S::LEAST * static_cast<int>(sizeof(T)); }
-    __device__ __forceinline__ void wait_for_queries(int row_bytes) {
+    __device__ __forceinline__ void wait_for_queries(int row_bytes, bool negative) {
+        const uint32_t sign = !negative ? 0u : sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 if (maybe_behind(c) && 64 * c + 16 * static_cast<int>(threadIdx.x % 64 / 16) >= row_bytes) q[rt][c] = make_uint4(0, 0, 0, 0);
+                q[rt][c].x ^= sign; q[rt][c].y ^= sign; q[rt][c].z ^= sign; q[rt][c].w ^= sign;
                 asm volatile("" : "+v"(q[rt][c].x), "+v"(q[rt][c].y), "+v"(q[rt][c].z), "+v"(q[rt][c].w));
             }
     }
@@ -143,28 +147,31 @@ struct Rows {
     template <bool ONE_BY_ONE, typename V, typename W, typename F>
     __device__ __forceinline__ static void weigh(V&& word, W&& weight, F&& into) {
         if constexpr (sizeof(T) == 2) {
-            uint4 pb[RT];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-                pb[rt] = make_uint4(pack_bf16x2(weight(rt, 0), weight(rt, 1)), pack_bf16x2(weight(rt, 2), weight(rt, 3)), pack_bf16x2(weight(rt, 4), weight(rt, 5)),
-                                    pack_bf16x2(weight(rt, 6), weight(rt, 7)));
+            for (int h = 0; h < 4 * KT; h += 8) {
+                uint4 pb[RT];
 #pragma unroll
-            for (int w = 0; w < CH; ++w) {
-                uint32_t vw[8];
+                for (int rt = 0; rt < RT; ++rt)
+                    pb[rt] = make_uint4(pack_bf16x2(weight(rt, h), weight(rt, h + 1)), pack_bf16x2(weight(rt, h + 2), weight(rt, h + 3)),
+                                        pack_bf16x2(weight(rt, h + 4), weight(rt, h + 5)), pack_bf16x2(weight(rt, h + 6), weight(rt, h + 7)));
 #pragma unroll
-                for (int j = 0; j < 8; ++j) vw[j] = word(j, w);
+                for (int w = 0; w < CH; ++w) {
+                    uint32_t vw[8];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t sel = e == 0 ? 0x05040100u : 0x07060302u;
-                    const uint4 va = make_uint4(__builtin_amdgcn_perm(vw[1], vw[0], sel), __builtin_amdgcn_perm(vw[3], vw[2], sel),
-                                                __builtin_amdgcn_perm(vw[5], vw[4], sel), __builtin_amdgcn_perm(vw[7], vw[6], sel));
+                    for (int j = 0; j < 8; ++j) vw[j] = word(h + j, w);
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-                        into(2 * w + e, rt, [&](f32x4 c) {
-                            return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, pb[rt]), c, 0, 0, 0);
-                        });
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t sel = e == 0 ? 0x05040100u : 0x07060302u;
+                        const uint4 va = make_uint4(__builtin_amdgcn_perm(vw[1], vw[0], sel), __builtin_amdgcn_perm(vw[3], vw[2], sel),
+                                                    __builtin_amdgcn_perm(vw[5], vw[4], sel), __builtin_amdgcn_perm(vw[7], vw[6], sel));
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+                            into(2 * w + e, rt, [&](f32x4 c) {
+                                return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, pb[rt]), c, 0, 0, 0);
+                            });
+                    }
+                    if (ONE_BY_ONE) __builtin_amdgcn_sched_barrier(0);
                 }
-                if (ONE_BY_ONE) __builtin_amdgcn_sched_barrier(0);
             }
         } else {
 #pragma unroll
@@ -184,38 +191,35 @@ struct Rows {
         }
     }
 
-    // The scores of a tile's keys, in base 2. keys(kt, k) gives the lane's operands.
-    template <typename K>
-    __device__ __forceinline__ void scores(float (&p)[RT][4 * KT], float scale_log2e, int row_bytes, K&& keys) const {
+    // The products of a tile's keys (the lane's operands k) with the queries.
+    __device__ __forceinline__ void scores(float (&p)[RT][4 * KT], int row_bytes, uint4 (&k)[KT][CH]) const {
         const int G = threadIdx.x % 64 / 16;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
-            uint4 k[CH];
-            keys(kt, k);
 #pragma unroll
             for (int c = 0; c < CH; ++c)
-                if (maybe_behind(c) && 64 * c + 16 * G >= row_bytes) k[c] = make_uint4(0, 0, 0, 0);
+                if (maybe_behind(c) && 64 * c + 16 * G >= row_bytes) k[kt][c] = make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 f32x4 s{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
                     if constexpr (sizeof(T) == 2) {
-                        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[c]), __builtin_bit_cast(bf16x8, q[rt][c]), s, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[kt][c]), __builtin_bit_cast(bf16x8, q[rt][c]), s, 0, 0, 0);
                     } else {
-                        const f32x4 kf = __builtin_bit_cast(f32x4, k[c]), qf = __builtin_bit_cast(f32x4, q[rt][c]);
+                        const f32x4 kf = __builtin_bit_cast(f32x4, k[kt][c]), qf = __builtin_bit_cast(f32x4, q[rt][c]);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[i], qf[i], s, 0, 0, 0);
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p[rt][4 * kt + i] = s[i] * scale_log2e;
+                for (int i = 0; i < 4; ++i) p[rt][4 * kt + i] = s[i];
             }
         }
     }
-    // Scores to weights. The maximum that weights are taken against follows only when one lies 8 above it: weights then reach 2^8, which costs
+    // Products to weights 2^(scale p - ref), scale > 0 (what is not seen is -inf). The maximum that weights are taken against follows only when one lies 8 above it: weights then reach 2^8, which costs
     // no accuracy, and most tiles leave sums and outputs as they are.
-    __device__ __forceinline__ void weights(float (&p)[RT][4 * KT]) {
+    __device__ __forceinline__ void weights(float (&p)[RT][4 * KT], float scale) {
         float fix[RT];
         bool any = false;
 #pragma unroll
@@ -223,7 +227,7 @@ struct Rows {
             float mx = p[rt][0];
 #pragma unroll
             for (int j = 1; j < 4 * KT; ++j) mx = fmaxf(mx, p[rt][j]);
-            mx = rows_max(mx);
+            mx = rows_max(mx) * scale;
             const bool more = mx > m[rt] + 8.f;
             fix[rt] = more ? exp2_for<T>(m[rt] - mx) : 1.f;
             m[rt] = more ? mx : m[rt];
@@ -242,39 +246,36 @@ struct Rows {
             float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < 4 * KT; ++j) {
-                p[rt][j] = exp2_for<T>(p[rt][j] - ref[rt]);
+                p[rt][j] = exp2_for<T>(fmaf(p[rt][j], scale, -ref[rt]));
                 sum += p[rt][j];
             }
             l[rt] += sum;
         }
     }
 
-    // A tile whose keys all rows see.
-    template <typename K, typename V>
-    __device__ __forceinline__ void take(float scale_log2e, int row_bytes, K&& keys, V&& values) {
-        float p[RT][4 * KT];
-        scores(p, scale_log2e, row_bytes, keys);
-        uint32_t v[4 * KT][CH];
-        values(v);
-        weights(p);
+    // A tile whose keys all rows see, from its products on, with the lane's words of its values.
+    __device__ __forceinline__ void take(float (&p)[RT][4 * KT], float scale, const uint32_t (&v)[4 * KT][CH]) {
+        weights(p, scale);
         weigh<false>([&](int j, int w) { return v[j][w]; }, [&](int rt, int j) { return p[rt][j]; },
                      [&](int x, int rt, auto&& product) { o[x][rt] = product(o[x][rt]); });
     }
     // Any tile: keys [at0, at0 + KEYS) of the cache, or of the nodes; `valid` has a bit for each that exists. stored(j, w) gives a word of the values.
-    template <typename K, typename W>
-    __device__ __forceinline__ void take_some(const TreeAttentionParams& a, bool of_nodes, int at0, unsigned valid, int first, int nodes, int row_bytes, K&& keys, W&& stored) {
+    template <typename W>
+    __device__ __forceinline__ void take_some(float (&p)[RT][4 * KT], const TreeAttentionParams& a, bool of_nodes, int at0, unsigned long long valid, int first, int nodes,
+                                              W&& stored) {
         const int G = threadIdx.x % 64 / 16;
-        float p[RT][4 * KT];
-        scores(p, a.scale_log2e, row_bytes, keys);
         unsigned mine = 0;                   // which of the lane's keys exist
 #pragma unroll
-        for (int j = 0; j < 4 * KT; ++j) mine |= (valid >> (16 * (j / 4) + 4 * G + j % 4) & 1) << j;
+        for (int kt = 0; kt < KT; ++kt) mine |= static_cast<unsigned>(valid >> (16 * kt + 4 * G) & 15) << (4 * kt);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             unsigned seen = mine;
             if (of_nodes) {
-                const unsigned bits = static_cast<unsigned>(a.ancestors[static_cast<size_t>(token[rt]) * a.words + at0 / 64] >> (at0 % 64)) >> (4 * G);
-                seen &= (bits & 15u) | (KT == 2 ? (bits >> 16 & 15u) << 4 : 0u);
+                const unsigned long long bits = a.ancestors[static_cast<size_t>(token[rt]) * a.words + at0 / 64] >> (at0 % 64 + 4 * G);
+                unsigned above = 0;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) above |= static_cast<unsigned>(bits >> (16 * kt) & 15) << (4 * kt);
+                seen &= above;
             }
             if (a.window > 0)
 #pragma unroll
@@ -286,7 +287,7 @@ struct Rows {
 #pragma unroll
             for (int j = 0; j < 4 * KT; ++j) p[rt][j] = seen >> j & 1 ? p[rt][j] : -INFINITY;
         }
-        weights(p);
+        weights(p, a.scale);
         // A key that does not exist has some other row's values. A value that is not finite, in a tile of which some rows see less than others,
         // would reach those that do not see it as zero times it: the finite values are weighed as ever, and whether a row gives weight to a NaN,
         // +inf or -inf of a column is a product of ones and zeros. (The words are read anew for each, which keeps them out of the registers.)
@@ -355,34 +356,35 @@ __device__ __forceinline__ float2* split_state(const TreeAttentionParams& a, siz
 // 16-byte piece p of row k of a stage lies at piece p ^ k (rotated by k where a row's pieces are no power of two), so that 16 lanes that
 // read one piece of 16 rows meet no bank twice.
 constexpr int TABLE_ENTRIES = 2048;
-template <typename T, int NT, int NW, int KG>
+template <typename T, int NT, int K16, int NW, int KG>
 struct Stage {
-    using S = Shape<T, NT>;
+    using S = Shape<T, NT, K16>;
     static constexpr int ROW = S::CH * 64, PIECES = 4 * S::CH, LEAST = S::KEYS * KG;      // a key group has one tile of a stage at least
-    static constexpr int keys() {          // 16 KB of keys and values at least, in whole instructions of all wavefronts
+    static constexpr int keys() {          // 24 KB of keys and values at least, in whole instructions of all wavefronts
         int n = LEAST;
-        while (n * 2 * ROW < 16384 || n * PIECES % (64 * NW) != 0) n *= 2;
+        while (n * 2 * ROW < 24576 || n * PIECES % (64 * NW) != 0) n *= 2;
         return n;
     }
     static constexpr int KEYS = keys();
     static constexpr int MATRIX = KEYS * ROW, BYTES = 2 * MATRIX;
-    static constexpr int NUMBER = 5 * BYTES <= 81920 ? 5 : 4 * BYTES <= 81920 ? 4 : 3 * BYTES <= 131072 ? 3 : 2;
+    static constexpr int NUMBER = 4 * BYTES <= 131072 ? 4 : 3;            // one is read, the next has come, the others are on their way
     static constexpr int LOADS = KEYS * PIECES / 64 / NW;                 // of a wavefront, a stage and matrix
     static_assert(LOADS * 64 * NW == KEYS * PIECES, "whole instructions");
-    static constexpr int WORDS = (KEYS + 63) / 64;
+    static constexpr int MINE = KEYS / NW, PER_LOAD = 64 / PIECES;        // rows of a wavefront (it loads these), rows of a load instruction (0: less than one)
+    static_assert(MINE <= 64 && KEYS % NW == 0, "a bit a row");
 };
 
-template <typename T, int NT, int RT, int NW, int KG>
+template <typename T, int NT, int RT, int K16, int NW, int KG>
 __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionParams a) {
-    using R = Rows<T, NT, RT>;
-    using S = Shape<T, NT>;
-    using St = Stage<T, NT, NW, KG>;
+    using R = Rows<T, NT, RT, K16>;
+    using S = Shape<T, NT, K16>;
+    using St = Stage<T, NT, K16, NW, KG>;
     constexpr int KT = S::KT, KEYS = S::KEYS, CH = S::CH, TILES = S::TILES, PIECES = St::PIECES, SK = St::KEYS, RG = NW / KG, PITCH = 32 * NT + 4;
     constexpr bool POW2 = (PIECES & (PIECES - 1)) == 0;
     // the stages [keys, values][SK][PIECES * 16]; at the end the states [wavefront][16 RT][PITCH], then their maxima and sums
     extern __shared__ __attribute__((aligned(16))) unsigned char stage_s[];
     __shared__ int table_s[TABLE_ENTRIES];
-    __shared__ unsigned long long valid_s[St::NUMBER][St::WORDS];         // a bit a key that exists
+    __shared__ unsigned long long valid_s[St::NUMBER][NW];                // of each wavefront's rows of a stage: a bit a key that exists
     Work w;
     if (!w.find(a, 16 * RT * RG)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
@@ -420,17 +422,48 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     R r;
     r.begin(a, first, w.rows, w.group, hk, row0, row_bytes);
     if (begin < cache_tiles) fill_table(min(block_of(a, (begin + first_tile) * SK), a.max_blocks - 1));
-    r.wait_for_queries(row_bytes);
+    r.wait_for_queries(row_bytes, a.negative);
 
     const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)stage_s));
     const size_t head = static_cast<size_t>(hk) * row_bytes;
-    // Asks for a stage. (All of the workgroup come here, behind a barrier after which nobody reads what it fills.)
+    // Asks for a stage. (All of the workgroup come here, behind a barrier after which nobody reads what it fills.) A wavefront has MINE
+    // neighbouring rows of it. Where each of its load instructions takes whole rows that lie in one page, and all of them exist, an instruction's
+    // address is the page's and an offset that the lane keeps: a few scalar instructions a load. Otherwise every lane finds its row.
+    constexpr bool WHOLE = St::PER_LOAD > 0 && 64 % PIECES == 0 && POW2;
+    constexpr unsigned long long ALL_MINE = St::MINE == 64 ? ~0ull : (1ull << (St::MINE % 64)) - 1;
+    static_assert(!WHOLE || SK / St::PER_LOAD <= 64, "a lane a page");
+    const bool in_pages = WHOLE && a.page_size % std::max(St::PER_LOAD, 1) == 0;
+    unsigned offset[St::LOADS];
+#pragma unroll
+    for (int i = 0; i < St::LOADS; ++i) {
+        const int k = wave * St::MINE + i * St::PER_LOAD + lane / PIECES, piece = (lane % PIECES) ^ (k & (PIECES - 1));
+        offset[i] = (lane / PIECES) * a.page_pitch + (16 * piece < row_bytes ? 16 * piece : 0);
+    }
+    unsigned good = 0;             // a bit a stage: all of its keys exist
     auto ask = [&](int tile) {
         const bool of_nodes = tile >= cache_tiles;
         const int at0 = (of_nodes ? tile - cache_tiles : tile + first_tile) * SK, place = tile % St::NUMBER;
-        int lane = threadIdx.x % 64;
-        asm volatile("" : "+v"(lane));         // (what follows from it is worked out here, not kept in registers over the whole loop)
+        good &= ~(1u << place);
         if (!of_nodes && block_of(a, min(at0 + SK, cached) - 1) >= base + filled) fill_table(block_of(a, at0));
+        const unsigned to = lds0 + place * St::BYTES + wave * St::LOADS * 1024;
+        if (WHOLE && in_pages && !of_nodes && at0 + SK <= cached) {
+            // lane i: the first row of instruction i; and the stage's page i, all of which have to exist
+            const int at = at0 + wave * St::MINE + min(lane, St::LOADS - 1) * St::PER_LOAD, block = block_of(a, at), block0 = block_of(a, at0);
+            const int entry = table_s[block - base], any = table_s[min(block0 + lane, block_of(a, at0 + SK - 1)) - base];
+            const unsigned long long from = static_cast<unsigned long long>(static_cast<unsigned>(entry * a.page_size + at - block * a.page_size)) * a.page_pitch;
+            if (__all(static_cast<unsigned>(any) < static_cast<unsigned>(a.n_pages))) {
+                const int low = static_cast<int>(from), high = static_cast<int>(from >> 32);
+#pragma unroll
+                for (int i = 0; i < St::LOADS; ++i) {
+                    const size_t row = static_cast<size_t>(static_cast<unsigned>(__builtin_amdgcn_readlane(high, i))) << 32 | static_cast<unsigned>(__builtin_amdgcn_readlane(low, i));
+                    load_to_lds(reinterpret_cast<const unsigned char*>(a.k_pages) + head + row, offset[i], to + 1024 * i);
+                    load_to_lds(reinterpret_cast<const unsigned char*>(a.v_pages) + head + row, offset[i], to + St::MATRIX + 1024 * i);
+                }
+                if (lane == 0) valid_s[place][wave] = ALL_MINE;
+                good |= 1u << place;
+                return;
+            }
+        }
         auto row_of = [&](int k, bool& there) {
             if (of_nodes) {
                 there = at0 + k < nodes;
@@ -440,25 +473,19 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             there = at0 + k < cached && static_cast<unsigned>(entry) < static_cast<unsigned>(a.n_pages);
             return there ? entry * a.page_size + at - block * a.page_size : 0;
         };
-#pragma unroll
-        for (int i = 0; i < St::WORDS; ++i)
-            if (i % NW == wave) {
-                bool there;
-                row_of(64 * i + lane % SK, there);
-                const unsigned long long bits = __ballot(there && lane < SK);
-                if (lane == 0) valid_s[place][i] = bits;
-            }
-        const unsigned to = lds0 + place * St::BYTES + wave * St::LOADS * 1024;
+        bool there;
+        row_of(wave * St::MINE + lane % St::MINE, there);
+        const unsigned long long bits = __ballot(there) & ALL_MINE;
+        if (lane == 0) valid_s[place][wave] = bits;
         const unsigned char* kb = reinterpret_cast<const unsigned char*>(of_nodes ? a.k : a.k_pages) + head;
         const unsigned char* vb = reinterpret_cast<const unsigned char*>(of_nodes ? a.v : a.v_pages) + head;
         const size_t k_pitch = of_nodes ? a.ldk : a.page_pitch, v_pitch = of_nodes ? a.ldv : a.page_pitch;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < St::LOADS; ++i) {
-            const int slot = (wave * St::LOADS + i) * 64 + lane, k = slot / PIECES, there = slot % PIECES;
-            const int piece = POW2 ? there ^ (k & (PIECES - 1)) : (there + PIECES - k % PIECES) % PIECES;
+            const int slot = (wave * St::LOADS + i) * 64 + lane, k = slot / PIECES, put = slot % PIECES;
+            const int piece = POW2 ? put ^ (k & (PIECES - 1)) : (put + PIECES - k % PIECES) % PIECES;
             const int off = 16 * piece < row_bytes ? 16 * piece : 0;
-            bool ignored;
-            const size_t row = row_of(k, ignored);
+            const size_t row = row_of(k, there);
             load_to_lds(kb, row * k_pitch + off, to + 1024 * i);
             load_to_lds(vb, row * v_pitch + off, to + St::MATRIX + 1024 * i);
         }
@@ -470,51 +497,72 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     // One loop over the wavefront's tiles of all stages: in two loops, one in the other, the outputs would be copied from the one's registers
     // to the other's for every tile. (A wavefront whose rows lie behind the last works on the last again, and writes nothing.)
     constexpr int TURNS = SK / KEYS / KG;
-    bool all_seen = false;
-    for (int step = 0; step < (end - begin) * TURNS; ++step) {
-        const int turn = step % TURNS, tile = begin + step / TURNS;
-        const bool of_nodes = tile >= cache_tiles;
-        const int at0 = (of_nodes ? tile - cache_tiles : tile + first_tile) * SK, place = tile % St::NUMBER;
-        if (turn == 0) {
-            // this stage has come (those behind it may be on their way), and all have read the one before it
-            wait_tiles_and_meet<St::NUMBER - 2, 2 * St::LOADS>(min(St::NUMBER - 2, end - 1 - tile));
-            if (tile + St::NUMBER - 1 < end) ask(tile + St::NUMBER - 1);
-            unsigned long long whole = ~0ull;
+    // Everything comes from LDS a phase before it is multiplied: a tile's keys while the tile in front of it is weighed (its stage has come by then),
+    // its values while its own products are made.
+    uint4 k[KT][CH];
+    auto read_keys = [&](int step) {
+        const int k0 = (step % TURNS * KG + kg) * KEYS;
+        const unsigned char* keys = stage_s + (begin + step / TURNS) % St::NUMBER * St::BYTES;
 #pragma unroll
-            for (int i = 0; i < St::WORDS; ++i) whole &= valid_s[place][i];
-            if (SK < 64) whole |= ~0ull << (SK % 64);
-            all_seen = !of_nodes && (a.window <= 0 || at0 >= r.low_most) && __builtin_amdgcn_readfirstlane(whole == ~0ull);
-        }
-        const unsigned char* keys = stage_s + place * St::BYTES;
-        const int k0 = (turn * KG + kg) * KEYS;
-        auto keys_of = [&](int kt, uint4 (&k)[CH]) {
+        for (int kt = 0; kt < KT; ++kt) {
             const int row = k0 + 16 * kt + c16;
 #pragma unroll
-            for (int c = 0; c < CH; ++c) k[c] = *reinterpret_cast<const uint4*>(keys + row * St::ROW + place_of(row, 4 * c + G));
-        };
-        if (all_seen) {
-            r.take(a.scale_log2e, row_bytes, keys_of, [&](uint32_t (&v)[4 * KT][CH]) {
+            for (int c = 0; c < CH; ++c) k[kt][c] = *reinterpret_cast<const uint4*>(keys + row * St::ROW + place_of(row, 4 * c + G));
+        }
+    };
+    const int steps = (end - begin) * TURNS;
+    if (steps > 0) {
+        wait_tiles_and_meet<St::NUMBER - 3, 2 * St::LOADS>(min(St::NUMBER - 3, end - 1 - begin));
+        read_keys(0);
+    }
+    for (int step = 0; step < steps; ++step) {
+        const int turn = step % TURNS, tile = begin + step / TURNS, place = tile % St::NUMBER;
+        const unsigned char* keys = stage_s + place * St::BYTES;
+        const int k0 = (turn * KG + kg) * KEYS;
+        if (turn == 0) {
+            // the next stage has come (those behind it may be on their way), and all have read the one in front of this
+            wait_tiles_and_meet<St::NUMBER - 3, 2 * St::LOADS>(max(0, min(St::NUMBER - 3, end - 2 - tile)));
+            if (tile + St::NUMBER - 1 < end) ask(tile + St::NUMBER - 1);
+        }
+        uint32_t v[4 * KT][CH];
 #pragma unroll
-                for (int j = 0; j < 4 * KT; ++j) {
-                    const int row = k0 + 16 * (j / 4) + 4 * G + j % 4;
-                    const unsigned char* at = keys + St::MATRIX + row * St::ROW;
+        for (int j = 0; j < 4 * KT; ++j) {
+            const int row = k0 + 16 * (j / 4) + 4 * G + j % 4;
+            const unsigned char* at = keys + St::MATRIX + row * St::ROW;
 #pragma unroll
-                    for (int x = 0; x < CH; x += S::block_words(x)) {
-                        if (S::block_words(x) == 4) {
-                            const uint4 u = *reinterpret_cast<const uint4*>(at + place_of(row, 4 * x + c16));
-                            v[j][x] = u.x; v[j][x + 1] = u.y; v[j][x + 2] = u.z; v[j][x + 3] = u.w;
-                        } else if (S::block_words(x) == 2) {
-                            const uint2 u = *reinterpret_cast<const uint2*>(at + place_of(row, 4 * x + c16 / 2) + 8 * (c16 % 2));
-                            v[j][x] = u.x; v[j][x + 1] = u.y;
-                        } else {
-                            v[j][x] = *reinterpret_cast<const uint32_t*>(at + place_of(row, 4 * x + c16 / 4) + 4 * (c16 % 4));
-                        }
-                    }
+            for (int x = 0; x < CH; x += S::block_words(x)) {
+                if (S::block_words(x) == 4) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(at + place_of(row, 4 * x + c16));
+                    v[j][x] = u.x; v[j][x + 1] = u.y; v[j][x + 2] = u.z; v[j][x + 3] = u.w;
+                } else if (S::block_words(x) == 2) {
+                    const uint2 u = *reinterpret_cast<const uint2*>(at + place_of(row, 4 * x + c16 / 2) + 8 * (c16 % 2));
+                    v[j][x] = u.x; v[j][x + 1] = u.y;
+                } else {
+                    v[j][x] = *reinterpret_cast<const uint32_t*>(at + place_of(row, 4 * x + c16 / 4) + 4 * (c16 % 4));
                 }
-            });
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        float p[RT][4 * KT];
+        r.scores(p, row_bytes, k);
+        __builtin_amdgcn_sched_barrier(0);
+        read_keys(min(step + 1, steps - 1));
+        __builtin_amdgcn_sched_barrier(0);
+        const bool of_nodes = tile >= cache_tiles;
+        const int at0 = (of_nodes ? tile - cache_tiles : tile + first_tile) * SK;
+        if ((good >> place & 1) && (a.window <= 0 || at0 >= r.low_most)) {
+            r.take(p, a.scale, v);
         } else {
-            const unsigned some = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(valid_s[place][k0 / 64] >> (k0 % 64))) & R::ALL;
-            r.take_some(a, of_nodes, at0 + k0, some, first, nodes, row_bytes, keys_of, [&](int j, int x) {
+            unsigned long long some = 0;
+            if (St::MINE >= KEYS) {
+                some = valid_s[place][k0 / St::MINE] >> (k0 % St::MINE) & R::ALL;
+            } else {
+#pragma unroll
+                for (int i = 0; i < KEYS / St::MINE; ++i) some |= valid_s[place][k0 / St::MINE + i] << (i * St::MINE);
+            }
+            some = static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(some >> 32)))) << 32 |
+                   static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(some)));
+            r.take_some(p, a, of_nodes, at0 + k0, some, first, nodes, [&](int j, int x) {
                 const int row = k0 + 16 * (j / 4) + 4 * G + j % 4, n = S::block_words(x), byte = 64 * S::block_first(x) + 4 * n * c16 + 4 * (x % n);
                 return *reinterpret_cast<const uint32_t*>(keys + St::MATRIX + row * St::ROW + place_of(row, byte / 16) + byte % 16);
             });
@@ -639,33 +687,31 @@ Plan plan_of(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_new,
     if (p.nt == 5) p.nt = 6;
     if (p.nt == 7) p.nt = 8;
     const long long rows = static_cast<long long>(max_new) * (n_heads / n_kv_heads);
-    const int most = p.nt <= 2 ? 8 : p.nt <= 4 ? 4 : 2;          // key groups whose stage fits twice
+    // Key groups: as many as there is a 32-KB stage for (at most 8 wavefronts).
     p.rt = 1;
-    int row_groups = 1;
-    if (rows > 16) row_groups = 2;
-    if (rows > 32) row_groups = 4;
-    if (rows > 64) { row_groups = p.nt <= 4 ? 4 : 8; p.rt = p.nt <= 4 ? 2 : 1; }
-    if (rows > 128 && p.nt <= 4) row_groups = 8;
-    p.waves = p.nt <= 2 ? 8 : std::min(8, row_groups * most);
-    p.key_groups = p.waves / row_groups;
+    int row_groups = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8;
+    if (p.nt <= (f32 ? 2 : 4) && rows > 64) { p.rt = 2; row_groups = rows <= 128 ? 4 : 8; }
+    if (p.nt == 8) row_groups = std::min(row_groups, 4);        // (registers)
+    p.key_groups = std::min(p.nt <= 2 ? 4 : p.nt <= 4 ? 2 : 1, 8 / row_groups);
+    p.waves = row_groups * p.key_groups;
     const int each = 16 * p.rt * row_groups;
     p.row_tiles = static_cast<int>((rows + each - 1) / each);
     const int keys = f32 ? 16 : 32;
     const long long seen = window > 0 ? std::min<long long>(max_cached, static_cast<long long>(window) + max_new) : max_cached;
     const long long tiles = (seen + keys - 1) / keys + (max_new + keys - 1) / keys;
     const long long groups = static_cast<long long>(n_seqs) * n_kv_heads * p.row_tiles;
-    p.nsplit = static_cast<int>(std::max<long long>(1, std::min<long long>({512 / groups, tiles / (4 * p.key_groups), 64})));
+    p.nsplit = static_cast<int>(std::max<long long>(1, std::min<long long>({256 / groups, tiles / (4 * p.key_groups), 64})));
     return p;
 }
 
-template <typename T, int NT, int RT, int NW, int KG>
+template <typename T, int NT, int RT, int K16, int NW, int KG>
 int launch(const TreeAttentionParams& p, hipStream_t stream) {
-    using St = Stage<T, NT, NW, KG>;
+    using St = Stage<T, NT, K16, NW, KG>;
     const long long blocks = (static_cast<long long>(p.units) + 7) / 8 * 8 * p.row_tiles;
     if (blocks > INT32_MAX) return -1;
     constexpr int STATES = KG == 1 ? 0 : NW * 16 * RT * ((32 * NT + 4) * 4 + 8), LDS = std::max(St::NUMBER * St::BYTES, STATES);
     static_assert(LDS + TABLE_ENTRIES * 4 + 1024 <= 163840, "LDS of a compute unit");
-    auto kernel = tree_attention_kernel<T, NT, RT, NW, KG>;
+    auto kernel = tree_attention_kernel<T, NT, RT, K16, NW, KG>;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (e != hipSuccess) return static_cast<int>(e);
     kernel<<<static_cast<unsigned>(blocks), NW * 64, LDS, stream>>>(p);
@@ -674,11 +720,20 @@ int launch(const TreeAttentionParams& p, hipStream_t stream) {
 
 template <typename T>
 int dispatch(const TreeAttentionParams& p, const Plan& plan, hipStream_t stream) {
-#define TREE_CASE(N, R, W, K) if (plan.nt == N && plan.rt == R && plan.waves == W && plan.key_groups == K) return launch<T, N, R, W, K>(p, stream);
-#define TREE_NARROW(N) TREE_CASE(N, 1, 8, 8) TREE_CASE(N, 1, 8, 4) TREE_CASE(N, 1, 8, 2) TREE_CASE(N, 2, 8, 2) TREE_CASE(N, 2, 8, 1)
-#define TREE_MIDDLE(N) TREE_CASE(N, 1, 4, 4) TREE_CASE(N, 1, 8, 4) TREE_CASE(N, 1, 8, 2) TREE_CASE(N, 2, 8, 2) TREE_CASE(N, 2, 8, 1)
-#define TREE_WIDE(N) TREE_CASE(N, 1, 2, 2) TREE_CASE(N, 1, 4, 2) TREE_CASE(N, 1, 8, 2) TREE_CASE(N, 1, 8, 1)
+    // (16-key groups of a tile: as many as the registers hold beside the outputs where few wavefronts share the keys, so that there is independent
+    // work for the latencies from keys to outputs; where many do, as few as one product takes, so that a stage is not too large)
+    constexpr int ONE = sizeof(T) == 2 ? 2 : 1, TWO = sizeof(T) == 2 ? 4 : 2;
+#define TREE_CASE(N, R, K, W, G) if (plan.nt == N && plan.rt == R && plan.waves == W && plan.key_groups == G) return launch<T, N, R, K, W, G>(p, stream);
+#define TREE_NARROW(N) TREE_CASE(N, 1, ONE, 4, 4) TREE_CASE(N, 1, ONE, 8, 4) TREE_CASE(N, 1, TWO, 8, 2) TREE_CASE(N, 2, ONE, 8, 2) TREE_CASE(N, 2, ONE, 8, 1)
+#define TREE_MIDDLE(N) TREE_CASE(N, 1, ONE, 2, 2) TREE_CASE(N, 1, ONE, 4, 2) TREE_CASE(N, 1, ONE, 8, 2)
+#define TREE_WIDE(N) TREE_CASE(N, 1, ONE, 1, 1) TREE_CASE(N, 1, ONE, 2, 1) TREE_CASE(N, 1, ONE, 4, 1)
     TREE_NARROW(1) TREE_NARROW(2) TREE_MIDDLE(3) TREE_MIDDLE(4) TREE_WIDE(6) TREE_WIDE(8)
+    TREE_CASE(6, 1, ONE, 8, 1)
+    if constexpr (sizeof(T) == 2) {
+        TREE_CASE(3, 2, ONE, 8, 2) TREE_CASE(3, 2, ONE, 8, 1) TREE_CASE(4, 2, ONE, 8, 2) TREE_CASE(4, 2, ONE, 8, 1)
+    } else {
+        TREE_CASE(3, 1, ONE, 8, 1) TREE_CASE(4, 1, ONE, 8, 1)
+    }
 #undef TREE_WIDE
 #undef TREE_MIDDLE
 #undef TREE_NARROW
@@ -721,7 +776,9 @@ int mllm_tree_attention(const void* q, long long ldq, const void* k, long long l
     p.page_shift = 31 + bits;
     p.page_magic = static_cast<unsigned>(((1ull << p.page_shift) + page_size - 1) / page_size);
     p.row_tiles = plan.row_tiles; p.nsplit = plan.nsplit; p.units = static_cast<int>(units);
-    p.scale_log2e = scale * MLLM_LOG2E;
+    // (a scale of zero: so small that every finite product becomes zero by it, and -inf stays)
+    p.scale = std::max(std::fabs(scale) * MLLM_LOG2E, 1e-37f);
+    p.negative = scale < 0.f;
     p.out = static_cast<char*>(out); p.ws = ws;
     const int rc = dtype == MLLM_F32 ? dispatch<float>(p, plan, stream) : dispatch<bf16_t>(p, plan, stream);
     if (rc != 0) return rc;
