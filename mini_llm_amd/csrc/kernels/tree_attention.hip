@@ -89,7 +89,8 @@ struct Rows {
 
     uint4 q[RT][CH];
     f32x4 o[TILES][RT];
-    float m[RT], ref[RT], l[RT];
+    f32x4 sum[RT];                     // of the weights: bfloat16: in every element, of all lanes' keys; 32 bits: in the first, of the lane's
+    float m[RT], ref[RT];              // the same in the four lanes of a row
     int low[RT], token[RT];            // (what stands in front of `low` is not seen)
     int low_least, low_most;
 
@@ -118,12 +119,12 @@ struct Rows {
                 low_least = min(low_least, __shfl_xor(low_least, off, 64));
                 low_most = max(low_most, __shfl_xor(low_most, off, 64));
             }
-            low_least = __builtin_amdgcn_readfirstlane(low_least);
-            low_most = __builtin_amdgcn_readfirstlane(low_most);
         }
+        low_least = __builtin_amdgcn_readfirstlane(low_least);
+        low_most = __builtin_amdgcn_readfirstlane(low_most);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            m[rt] = -INFINITY; ref[rt] = 0.f; l[rt] = 0.f;
+            m[rt] = -INFINITY; ref[rt] = 0.f; sum[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int x = 0; x < TILES; ++x) o[x][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
@@ -144,8 +145,9 @@ struct Rows {
 
     // The second product: into(x, rt, product) for every tile x of columns and 16 rows, of the words word(j, w) of the lane's keys j and the weights
     // weight(rt, j).
-    template <bool ONE_BY_ONE, typename V, typename W, typename F>
-    __device__ __forceinline__ static void weigh(V&& word, W&& weight, F&& into) {
+    // In bfloat16 added(rt, product) is handed the product of ones with the weights, whose rows are the weights' sum.
+    template <bool ONE_BY_ONE, typename V, typename W, typename F, typename A>
+    __device__ __forceinline__ static void weigh(V&& word, W&& weight, F&& into, A&& added) {
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
             for (int h = 0; h < 4 * KT; h += 8) {
@@ -154,6 +156,12 @@ struct Rows {
                 for (int rt = 0; rt < RT; ++rt)
                     pb[rt] = make_uint4(pack_bf16x2(weight(rt, h), weight(rt, h + 1)), pack_bf16x2(weight(rt, h + 2), weight(rt, h + 3)),
                                         pack_bf16x2(weight(rt, h + 4), weight(rt, h + 5)), pack_bf16x2(weight(rt, h + 6), weight(rt, h + 7)));
+                const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                    added(rt, [&](f32x4 c) {
+                        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones), __builtin_bit_cast(bf16x8, pb[rt]), c, 0, 0, 0);
+                    });
 #pragma unroll
                 for (int w = 0; w < CH; ++w) {
                     uint32_t vw[8];
@@ -194,11 +202,14 @@ struct Rows {
     // The products of a tile's keys (the lane's operands k) with the queries.
     __device__ __forceinline__ void scores(float (&p)[RT][4 * KT], int row_bytes, uint4 (&k)[KT][CH]) const {
         const int G = threadIdx.x % 64 / 16;
+        if (row_bytes != 64 * CH)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int c = 0; c < CH; ++c)
+                    if (maybe_behind(c) && 64 * c + 16 * G >= row_bytes) k[kt][c] = make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
-#pragma unroll
-            for (int c = 0; c < CH; ++c)
-                if (maybe_behind(c) && 64 * c + 16 * G >= row_bytes) k[kt][c] = make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 f32x4 s{0.f, 0.f, 0.f, 0.f};
@@ -217,47 +228,47 @@ struct Rows {
             }
         }
     }
-    // Products to weights 2^(scale p - ref), scale > 0 (what is not seen is -inf). The maximum that weights are taken against follows only when one lies 8 above it: weights then reach 2^8, which costs
-    // no accuracy, and most tiles leave sums and outputs as they are.
+    // Products to weights 2^(scale p - ref), scale > 0 (what is not seen is -inf). The maximum that weights are taken against follows only when
+    // a product lies 8 above it: weights then reach 2^8, which costs no accuracy, and most tiles leave sums and outputs as they are and
+    // need not know the maximum over a row's four lanes.
     __device__ __forceinline__ void weights(float (&p)[RT][4 * KT], float scale) {
-        float fix[RT];
+        float mx[RT];
         bool any = false;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            float mx = p[rt][0];
+            mx[rt] = p[rt][0];
 #pragma unroll
-            for (int j = 1; j < 4 * KT; ++j) mx = fmaxf(mx, p[rt][j]);
-            mx = rows_max(mx) * scale;
-            const bool more = mx > m[rt] + 8.f;
-            fix[rt] = more ? exp2_for<T>(m[rt] - mx) : 1.f;
-            m[rt] = more ? mx : m[rt];
-            ref[rt] = more ? mx : ref[rt];
-            any = any || more;
+            for (int j = 1; j < 4 * KT; ++j) mx[rt] = fmaxf(mx[rt], p[rt][j]);
+            mx[rt] *= scale;
+            any |= mx[rt] > m[rt] + 8.f;
         }
         if (__any(any))
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                l[rt] *= fix[rt];
+                const float top = rows_max(mx[rt]);
+                const bool more = top > m[rt] + 8.f;
+                const float fix = more ? exp2_for<T>(m[rt] - top) : 1.f;
+                m[rt] = more ? top : m[rt];
+                ref[rt] = more ? top : ref[rt];
+                sum[rt] *= fix;
 #pragma unroll
-                for (int x = 0; x < TILES; ++x) o[x][rt] *= fix[rt];
+                for (int x = 0; x < TILES; ++x) o[x][rt] *= fix;
             }
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            float sum = 0.f;
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int j = 0; j < 4 * KT; ++j) {
                 p[rt][j] = exp2_for<T>(fmaf(p[rt][j], scale, -ref[rt]));
-                sum += p[rt][j];
+                if (sizeof(T) == 4) sum[rt][0] += p[rt][j];
             }
-            l[rt] += sum;
-        }
     }
+    __device__ __forceinline__ float sum_of(int rt) const { return sizeof(T) == 4 ? rows_sum(sum[rt][0]) : sum[rt][0]; }
 
     // A tile whose keys all rows see, from its products on, with the lane's words of its values.
     __device__ __forceinline__ void take(float (&p)[RT][4 * KT], float scale, const uint32_t (&v)[4 * KT][CH]) {
         weights(p, scale);
         weigh<false>([&](int j, int w) { return v[j][w]; }, [&](int rt, int j) { return p[rt][j]; },
-                     [&](int x, int rt, auto&& product) { o[x][rt] = product(o[x][rt]); });
+                     [&](int x, int rt, auto&& product) { o[x][rt] = product(o[x][rt]); }, [&](int rt, auto&& product) { sum[rt] = product(sum[rt]); });
     }
     // Any tile: keys [at0, at0 + KEYS) of the cache, or of the nodes; `valid` has a bit for each that exists. stored(j, w) gives a word of the values.
     template <typename W>
@@ -303,7 +314,7 @@ struct Rows {
         }
         asm volatile("" ::: "memory");
         const bool special = __any(odd != 0);
-        weigh<true>([&](int j, int w) { return special ? sifted(word(j, w), 0, T{}) : word(j, w); }, weight, add);
+        weigh<true>([&](int j, int w) { return special ? sifted(word(j, w), 0, T{}) : word(j, w); }, weight, add, [&](int rt, auto&& product) { sum[rt] = product(sum[rt]); });
         if (!special) return;
 #pragma unroll 1
         for (int kind = 1; kind <= 3; ++kind) {
@@ -314,7 +325,7 @@ struct Rows {
                             const f32x4 count = product(f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
                             for (int i = 0; i < 4; ++i) o[x][rt][i] += count[i] > 0.f ? value : 0.f;
-                        });
+                        }, [](int, auto&&) {});
         }
     }
 
@@ -353,7 +364,7 @@ __device__ __forceinline__ float2* split_state(const TreeAttentionParams& a, siz
     return reinterpret_cast<float2*>(a.ws + static_cast<size_t>(a.tokens) * a.n_heads * a.nsplit * a.head_dim) + pair;
 }
 
-// 16-byte piece p of row k of a stage lies at piece p ^ k (rotated by k where a row's pieces are no power of two), so that 16 lanes that
+// 16-byte piece p of row k of a stage lies at piece p ^ (k % 16) (rotated by it where a row's pieces are no power of two), so that 16 lanes that
 // read one piece of 16 rows meet no bank twice.
 constexpr int TABLE_ENTRIES = 2048;
 template <typename T, int NT, int K16, int NW, int KG>
@@ -381,6 +392,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     using St = Stage<T, NT, K16, NW, KG>;
     constexpr int KT = S::KT, KEYS = S::KEYS, CH = S::CH, TILES = S::TILES, PIECES = St::PIECES, SK = St::KEYS, RG = NW / KG, PITCH = 32 * NT + 4;
     constexpr bool POW2 = (PIECES & (PIECES - 1)) == 0;
+    constexpr int TURN = std::min(PIECES, 16) - 1;
     // the stages [keys, values][SK][PIECES * 16]; at the end the states [wavefront][16 RT][PITCH], then their maxima and sums
     extern __shared__ __attribute__((aligned(16))) unsigned char stage_s[];
     __shared__ int table_s[TABLE_ENTRIES];
@@ -436,13 +448,13 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     unsigned offset[St::LOADS];
 #pragma unroll
     for (int i = 0; i < St::LOADS; ++i) {
-        const int k = wave * St::MINE + i * St::PER_LOAD + lane / PIECES, piece = (lane % PIECES) ^ (k & (PIECES - 1));
+        const int k = wave * St::MINE + i * St::PER_LOAD + lane / PIECES, piece = (lane % PIECES) ^ (k & TURN);
         offset[i] = (lane / PIECES) * a.page_pitch + (16 * piece < row_bytes ? 16 * piece : 0);
     }
     unsigned good = 0;             // a bit a stage: all of its keys exist
     auto ask = [&](int tile) {
         const bool of_nodes = tile >= cache_tiles;
-        const int at0 = (of_nodes ? tile - cache_tiles : tile + first_tile) * SK, place = tile % St::NUMBER;
+        const int at0 = (of_nodes ? tile - cache_tiles : tile + first_tile) * SK, place = static_cast<unsigned>(tile) % St::NUMBER;
         good &= ~(1u << place);
         if (!of_nodes && block_of(a, min(at0 + SK, cached) - 1) >= base + filled) fill_table(block_of(a, at0));
         const unsigned to = lds0 + place * St::BYTES + wave * St::LOADS * 1024;
@@ -483,14 +495,14 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
 #pragma unroll 1
         for (int i = 0; i < St::LOADS; ++i) {
             const int slot = (wave * St::LOADS + i) * 64 + lane, k = slot / PIECES, put = slot % PIECES;
-            const int piece = POW2 ? put ^ (k & (PIECES - 1)) : (put + PIECES - k % PIECES) % PIECES;
+            const int piece = POW2 ? put ^ (k & TURN) : (put + PIECES - k % 16 % PIECES) % PIECES;
             const int off = 16 * piece < row_bytes ? 16 * piece : 0;
             const size_t row = row_of(k, there);
             load_to_lds(kb, row * k_pitch + off, to + 1024 * i);
             load_to_lds(vb, row * v_pitch + off, to + St::MATRIX + 1024 * i);
         }
     };
-    auto place_of = [&](int k, int piece) { return 16 * (POW2 ? piece ^ (k & (PIECES - 1)) : (piece + k) % PIECES); };
+    auto place_of = [&](int k, int piece) { return 16 * (POW2 ? piece ^ (k & TURN) : (piece + k % 16) % PIECES); };
 
     for (int i = 0; i < St::NUMBER - 1; ++i)
         if (begin + i < end) ask(begin + i);
@@ -499,16 +511,26 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     constexpr int TURNS = SK / KEYS / KG;
     // Everything comes from LDS a phase before it is multiplied: a tile's keys while the tile in front of it is weighed (its stage has come by then),
     // its values while its own products are made.
-    uint4 k[KT][CH];
-    auto read_keys = [&](int step) {
-        const int k0 = (step % TURNS * KG + kg) * KEYS;
-        const unsigned char* keys = stage_s + (begin + step / TURNS) % St::NUMBER * St::BYTES;
+    int key_at[CH], value_at[4][CH];        // of the lane's pieces of 16 rows; those of the next 16 lie 16 rows behind
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            const int row = k0 + 16 * kt + c16;
+    for (int c = 0; c < CH; ++c) key_at[c] = c16 * St::ROW + place_of(c16, 4 * c + G);
 #pragma unroll
-            for (int c = 0; c < CH; ++c) k[kt][c] = *reinterpret_cast<const uint4*>(keys + row * St::ROW + place_of(row, 4 * c + G));
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int x = 0; x < CH; ++x) {
+            const int row = 4 * G + i, n = S::block_words(x), byte = 64 * S::block_first(x) + 4 * n * c16;
+            value_at[i][x] = St::MATRIX + row * St::ROW + place_of(row, byte / 16) + byte % 16;
         }
+    uint4 k[KT][CH];
+    auto tile_of = [&](int step) {
+        return stage_s + static_cast<unsigned>(begin + step / TURNS) % St::NUMBER * St::BYTES + (step % TURNS * KG + kg) * (KEYS * St::ROW);
+    };
+    auto read_keys = [&](int step) {
+        const unsigned char* keys = tile_of(step);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) k[kt][c] = *reinterpret_cast<const uint4*>(keys + key_at[c] + kt * 16 * St::ROW);
     };
     const int steps = (end - begin) * TURNS;
     if (steps > 0) {
@@ -516,8 +538,8 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
         read_keys(0);
     }
     for (int step = 0; step < steps; ++step) {
-        const int turn = step % TURNS, tile = begin + step / TURNS, place = tile % St::NUMBER;
-        const unsigned char* keys = stage_s + place * St::BYTES;
+        const int turn = step % TURNS, tile = begin + step / TURNS, place = static_cast<unsigned>(tile) % St::NUMBER;
+        const unsigned char* keys = tile_of(step);
         const int k0 = (turn * KG + kg) * KEYS;
         if (turn == 0) {
             // the next stage has come (those behind it may be on their way), and all have read the one in front of this
@@ -526,22 +548,20 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
         }
         uint32_t v[4 * KT][CH];
 #pragma unroll
-        for (int j = 0; j < 4 * KT; ++j) {
-            const int row = k0 + 16 * (j / 4) + 4 * G + j % 4;
-            const unsigned char* at = keys + St::MATRIX + row * St::ROW;
+        for (int j = 0; j < 4 * KT; ++j)
 #pragma unroll
             for (int x = 0; x < CH; x += S::block_words(x)) {
+                const unsigned char* at = keys + value_at[j % 4][x] + j / 4 * 16 * St::ROW;
                 if (S::block_words(x) == 4) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(at + place_of(row, 4 * x + c16));
+                    const uint4 u = *reinterpret_cast<const uint4*>(at);
                     v[j][x] = u.x; v[j][x + 1] = u.y; v[j][x + 2] = u.z; v[j][x + 3] = u.w;
                 } else if (S::block_words(x) == 2) {
-                    const uint2 u = *reinterpret_cast<const uint2*>(at + place_of(row, 4 * x + c16 / 2) + 8 * (c16 % 2));
+                    const uint2 u = *reinterpret_cast<const uint2*>(at);
                     v[j][x] = u.x; v[j][x + 1] = u.y;
                 } else {
-                    v[j][x] = *reinterpret_cast<const uint32_t*>(at + place_of(row, 4 * x + c16 / 4) + 4 * (c16 % 4));
+                    v[j][x] = *reinterpret_cast<const uint32_t*>(at);
                 }
             }
-        }
         __builtin_amdgcn_sched_barrier(0);
         float p[RT][4 * KT];
         r.scores(p, row_bytes, k);
@@ -550,7 +570,11 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
         __builtin_amdgcn_sched_barrier(0);
         const bool of_nodes = tile >= cache_tiles;
         const int at0 = (of_nodes ? tile - cache_tiles : tile + first_tile) * SK;
-        if ((good >> place & 1) && (a.window <= 0 || at0 >= r.low_most)) {
+        // (The condition is kept in a lane's register: as a scalar branch, which the same one in all lanes could be, the compiler gives the outputs other
+        // registers on either side of a product, and moves or spills them every time.)
+        int all_seen = (good >> place & 1) && (a.window <= 0 || at0 >= r.low_most);
+        asm volatile("" : "+v"(all_seen));
+        if (all_seen) {
             r.take(p, a.scale, v);
         } else {
             unsigned long long some = 0;
@@ -563,8 +587,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             some = static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(some >> 32)))) << 32 |
                    static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(some)));
             r.take_some(p, a, of_nodes, at0 + k0, some, first, nodes, [&](int j, int x) {
-                const int row = k0 + 16 * (j / 4) + 4 * G + j % 4, n = S::block_words(x), byte = 64 * S::block_first(x) + 4 * n * c16 + 4 * (x % n);
-                return *reinterpret_cast<const uint32_t*>(keys + St::MATRIX + row * St::ROW + place_of(row, byte / 16) + byte % 16);
+                return *reinterpret_cast<const uint32_t*>(keys + value_at[j % 4][x] + j / 4 * 16 * St::ROW + 4 * (x % S::block_words(x)));
             });
         }
     }
@@ -573,7 +596,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const int row = row0 + 16 * rt + c16;
-            const float sum = rows_sum(r.l[rt]);
+            const float sum = r.sum_of(rt);
             if (row >= w.rows) continue;
             const int node = row / w.group, t = first + node, h = hk * w.group + row - node * w.group;
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -602,7 +625,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     float2* ml_s = reinterpret_cast<float2*>(state_s + NW * 16 * RT * PITCH);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const float sum = rows_sum(r.l[rt]);
+        const float sum = r.sum_of(rt);
         if (G == 0) ml_s[wave * 16 * RT + 16 * rt + c16] = make_float2(r.m[rt], sum);
         float* to = state_s + (wave * 16 * RT + 16 * rt + c16) * PITCH;
 #pragma unroll
