@@ -80,6 +80,12 @@ __device__ __forceinline__ uint32_t sifted(uint32_t w, int kind, bf16_t) {
     return (special & (kind == 1 ? mantissa : ~mantissa & (kind == 2 ? ~sign : sign))) * 0x3f80u;
 }
 
+// What a row's weights are taken against before it has seen a key: finite, so that no difference of two of them is NaN.
+constexpr float LEAST_SCORE = -3.0e38f;
+
+// a / b for 0 <= a < 2^20, 1 <= b < 2^20, by the reciprocal: half a unit more than `a` lies further from the next quotient than it errs.
+__device__ __forceinline__ int lane_quotient(int a, int b) { return static_cast<int>((static_cast<float>(a) + 0.5f) * __builtin_amdgcn_rcpf(static_cast<float>(b))); }
+
 // One wavefront's rows, 16 RT of them, and what it has summed up for them.
 template <typename T, int NT, int RT, int KEY_GROUPS_OF_16>
 struct Rows {
@@ -90,8 +96,9 @@ struct Rows {
     uint4 q[RT][CH];
     f32x4 o[TILES][RT];
     f32x4 sum[RT];                     // of the weights: bfloat16: in every element, of all lanes' keys; 32 bits: in the first, of the lane's
-    float m[RT], ref[RT];              // the same in the four lanes of a row
+    float m[RT];                       // what weights are taken against, the same in the four lanes of a row
     int low[RT], token[RT];            // (what stands in front of `low` is not seen)
+    unsigned long long above[RT];      // the first word of the nodes seen (few rows: asked for ahead)
     int low_least, low_most;
 
     // Asks for the rows' queries (beyond the last: the last again, never written).
@@ -101,7 +108,7 @@ struct Rows {
         low_most = INT32_MIN;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const int r = min(row0 + 16 * rt + c16, rows - 1), node = r / group;
+            const int r = min(row0 + 16 * rt + c16, rows - 1), node = rows < 1 << 20 ? lane_quotient(r, group) : r / group;
             token[rt] = first + node;
             const char* at = a.q + token[rt] * a.ldq + (hk * group + r - node * group) * row_bytes;
 #pragma unroll
@@ -109,6 +116,7 @@ struct Rows {
                 const int off = 64 * c + 16 * G;
                 q[rt][c] = *reinterpret_cast<const uint4*>(at + (off < row_bytes ? off : 0));
             }
+            if (RT == 1) above[rt] = a.ancestors[static_cast<size_t>(token[rt]) * a.words];
             low[rt] = a.window > 0 ? a.positions[token[rt]] - a.window + 1 : INT32_MIN;
             low_least = min(low_least, low[rt]);
             low_most = max(low_most, low[rt]);
@@ -124,7 +132,7 @@ struct Rows {
         low_most = __builtin_amdgcn_readfirstlane(low_most);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            m[rt] = -INFINITY; ref[rt] = 0.f; sum[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            m[rt] = LEAST_SCORE; sum[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int x = 0; x < TILES; ++x) o[x][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
@@ -132,6 +140,9 @@ struct Rows {
     // Columns behind the head's last are zero in queries and keys.
     static constexpr bool maybe_behind(int c) { return 64 * (c + 1) > 32 * S::LEAST * static_cast<int>(sizeof(T)); }
     __device__ __forceinline__ void wait_for_queries(int row_bytes, bool negative) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+            if (RT == 1) asm volatile("" : "+v"(above[rt]));
         const uint32_t sign = !negative ? 0u : sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -228,7 +239,7 @@ struct Rows {
             }
         }
     }
-    // Products to weights 2^(scale p - ref), scale > 0 (what is not seen is -inf). The maximum that weights are taken against follows only when
+    // Products to weights 2^(scale p - m), scale > 0 (what is not seen is -inf). The maximum that weights are taken against follows only when
     // a product lies 8 above it: weights then reach 2^8, which costs no accuracy, and most tiles leave sums and outputs as they are and
     // need not know the maximum over a row's four lanes.
     __device__ __forceinline__ void weights(float (&p)[RT][4 * KT], float scale) {
@@ -249,7 +260,6 @@ struct Rows {
                 const bool more = top > m[rt] + 8.f;
                 const float fix = more ? exp2_for<T>(m[rt] - top) : 1.f;
                 m[rt] = more ? top : m[rt];
-                ref[rt] = more ? top : ref[rt];
                 sum[rt] *= fix;
 #pragma unroll
                 for (int x = 0; x < TILES; ++x) o[x][rt] *= fix;
@@ -258,7 +268,7 @@ struct Rows {
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int j = 0; j < 4 * KT; ++j) {
-                p[rt][j] = exp2_for<T>(fmaf(p[rt][j], scale, -ref[rt]));
+                p[rt][j] = exp2_for<T>(fmaf(p[rt][j], scale, -m[rt]));
                 if (sizeof(T) == 4) sum[rt][0] += p[rt][j];
             }
     }
@@ -270,10 +280,10 @@ struct Rows {
         weigh<false>([&](int j, int w) { return v[j][w]; }, [&](int rt, int j) { return p[rt][j]; },
                      [&](int x, int rt, auto&& product) { o[x][rt] = product(o[x][rt]); }, [&](int rt, auto&& product) { sum[rt] = product(sum[rt]); });
     }
-    // Any tile: keys [at0, at0 + KEYS) of the cache, or of the nodes; `valid` has a bit for each that exists. stored(j, w) gives a word of the values.
+    // Any tile: keys [at0, at0 + KEYS) of the cache, or of the nodes; `valid` has a bit for each that exists. stored(j, w) gives a word of the values again.
     template <typename W>
-    __device__ __forceinline__ void take_some(float (&p)[RT][4 * KT], const TreeAttentionParams& a, bool of_nodes, int at0, unsigned long long valid, int first, int nodes,
-                                              W&& stored) {
+    __device__ __forceinline__ void take_some(float (&p)[RT][4 * KT], const uint32_t (&v)[4 * KT][CH], const TreeAttentionParams& a, bool of_nodes, int at0,
+                                              unsigned long long valid, int first, int nodes, W&& stored) {
         const int G = threadIdx.x % 64 / 16;
         unsigned mine = 0;                   // which of the lane's keys exist
 #pragma unroll
@@ -282,11 +292,13 @@ struct Rows {
         for (int rt = 0; rt < RT; ++rt) {
             unsigned seen = mine;
             if (of_nodes) {
-                const unsigned long long bits = a.ancestors[static_cast<size_t>(token[rt]) * a.words + at0 / 64] >> (at0 % 64 + 4 * G);
-                unsigned above = 0;
+                unsigned long long bits = RT == 1 ? above[rt] : 0;
+                if (RT > 1 || at0 >= 64) bits = a.ancestors[static_cast<size_t>(token[rt]) * a.words + at0 / 64];
+                bits >>= at0 % 64 + 4 * G;
+                unsigned nodes_seen = 0;
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) above |= static_cast<unsigned>(bits >> (16 * kt) & 15) << (4 * kt);
-                seen &= above;
+                for (int kt = 0; kt < KT; ++kt) nodes_seen |= static_cast<unsigned>(bits >> (16 * kt) & 15) << (4 * kt);
+                seen &= nodes_seen;
             }
             if (a.window > 0)
 #pragma unroll
@@ -301,21 +313,27 @@ struct Rows {
         weights(p, a.scale);
         // A key that does not exist has some other row's values. A value that is not finite, in a tile of which some rows see less than others,
         // would reach those that do not see it as zero times it: the finite values are weighed as ever, and whether a row gives weight to a NaN,
-        // +inf or -inf of a column is a product of ones and zeros. (The words are read anew for each, which keeps them out of the registers.)
-        auto word = [&](int j, int w) { return stored(j, w) & (0u - (mine >> j & 1)); };
+        // +inf or -inf of a column is a product of ones and zeros. (For these products the words are read anew, which keeps them out of the registers.)
+        auto exists = [&](int j) { return 0u - (mine >> j & 1); };
         auto weight = [&](int rt, int j) { return p[rt][j]; };
         auto add = [&](int x, int rt, auto&& product) { o[x][rt] = product(o[x][rt]); };
         uint32_t odd = 0;
 #pragma unroll
-        for (int w = 0; w < CH; ++w) {
+        for (int j = 0; j < 4 * KT; ++j) {
+            uint32_t each = 0;
 #pragma unroll
-            for (int j = 0; j < 4 * KT; ++j) odd |= not_finite(word(j, w), T{});
-            __builtin_amdgcn_sched_barrier(0);
+            for (int w = 0; w < CH; ++w) each |= not_finite(v[j][w], T{});
+            odd |= each & exists(j);
         }
-        asm volatile("" ::: "memory");
         const bool special = __any(odd != 0);
-        weigh<true>([&](int j, int w) { return special ? sifted(word(j, w), 0, T{}) : word(j, w); }, weight, add, [&](int rt, auto&& product) { sum[rt] = product(sum[rt]); });
+        weigh<true>(
+            [&](int j, int w) {
+                uint32_t x = v[j][w] & exists(j);
+                return special ? sifted(x, 0, T{}) : x;
+            },
+            weight, add, [&](int rt, auto&& product) { sum[rt] = product(sum[rt]); });
         if (!special) return;
+        auto word = [&](int j, int w) { return stored(j, w) & exists(j); };
 #pragma unroll 1
         for (int kind = 1; kind <= 3; ++kind) {
             const float value = kind == 1 ? __builtin_nanf("") : kind == 2 ? INFINITY : -INFINITY;
@@ -342,17 +360,18 @@ struct Work {
     // Workgroups that share keys have numbers 8 apart, so that they run on one XCD and the second finds the keys in its L2.
     __device__ __forceinline__ bool find(const TreeAttentionParams& a, int rows_each) {
         const int residue = blockIdx.x % 8, rest = blockIdx.x / 8;
-        const int unit = rest / a.row_tiles * 8 + residue;
-        row_tile = rest % a.row_tiles;
+        const int eight = uniform_quotient(rest, a.row_tiles), unit = eight * 8 + residue;
+        row_tile = rest - eight * a.row_tiles;
         if (unit >= a.units) return false;
-        split = unit % a.nsplit;
-        hk = unit / a.nsplit % a.n_kv_heads;
-        b = unit / a.nsplit / a.n_kv_heads;
-        group = a.n_heads / a.n_kv_heads;
+        const int pair = uniform_quotient(unit, a.nsplit);
+        split = unit - pair * a.nsplit;
+        b = uniform_quotient(pair, a.n_kv_heads);
+        hk = pair - b * a.n_kv_heads;
+        group = small_quotient(a.n_heads, a.n_kv_heads);
         first = min(max(a.cu_q[b], 0), a.tokens);
         nodes = min(min(max(a.cu_q[b + 1] - first, 0), a.tokens - first), a.max_new);
         rows = nodes * group;
-        cached = static_cast<int>(min(min(static_cast<long long>(max(a.cached[b], 0)), static_cast<long long>(a.max_blocks) * a.page_size), INT32_MAX - 128ll));
+        cached = static_cast<int>(min(min(static_cast<long long>(max(a.cached[b], 0)), static_cast<long long>(a.max_blocks) * a.page_size), INT32_MAX - 65536ll));
         return row_tile * rows_each < rows;
     }
 };
@@ -405,14 +424,22 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     const int first = w.first, nodes = w.nodes, hk = w.hk, cached = w.cached;
     const int* table = a.block_tables + static_cast<size_t>(w.b) * a.max_blocks;
 
-    // A part of the block table lies in LDS, from entry `base` on; all of the workgroup meet here.
-    int base = 0, filled = 0;
+    // A part of the block table lies in LDS, from entry `base` on; all of the workgroup meet here. Whether all of its entries that the cache
+    // reaches name pages is known then.
+    int base = 0, filled = 0, all_pages = 0, ready = 0, ready_from = 0;
     auto fill_table = [&](int from) {
         lds_barrier();
         base = from;
         filled = min(TABLE_ENTRIES, a.max_blocks - from);
-        for (int i = threadIdx.x; i < filled; i += NW * 64) table_s[i] = table[from + i];
-        __syncthreads();
+        ready = 0;
+        const int reached = min(filled, block_of(a, cached - 1) + 1 - from);
+        int good = 1;
+        for (int i = threadIdx.x; i < filled; i += NW * 64) {
+            const int entry = table[from + i];
+            table_s[i] = entry;
+            good &= i >= reached || static_cast<unsigned>(entry) < static_cast<unsigned>(a.n_pages);
+        }
+        all_pages = __syncthreads_and(good);
     };
     // Tiles of SK keys: those of the cache from the window's first on, then the nodes'. A split has `per` neighbouring ones.
     int first_tile = 0;
@@ -443,7 +470,6 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     // address is the page's and an offset that the lane keeps: a few scalar instructions a load. Otherwise every lane finds its row.
     constexpr bool WHOLE = St::PER_LOAD > 0 && 64 % PIECES == 0 && POW2;
     constexpr unsigned long long ALL_MINE = St::MINE == 64 ? ~0ull : (1ull << (St::MINE % 64)) - 1;
-    static_assert(!WHOLE || SK / St::PER_LOAD <= 64, "a lane a page");
     const bool in_pages = WHOLE && a.page_size % std::max(St::PER_LOAD, 1) == 0;
     unsigned offset[St::LOADS];
 #pragma unroll
@@ -451,30 +477,34 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
         const int k = wave * St::MINE + i * St::PER_LOAD + lane / PIECES, piece = (lane % PIECES) ^ (k & TURN);
         offset[i] = (lane / PIECES) * a.page_pitch + (16 * piece < row_bytes ? 16 * piece : 0);
     }
+    // Where the first rows of AHEAD stages' instructions lie, from stage ready_from on: lane s * LOADS + i has instruction i of stage s.
+    constexpr int AHEAD = 64 / St::LOADS;
+    unsigned long long row_at = 0;
     unsigned good = 0;             // a bit a stage: all of its keys exist
     auto ask = [&](int tile) {
         const bool of_nodes = tile >= cache_tiles;
         const int at0 = (of_nodes ? tile - cache_tiles : tile + first_tile) * SK, place = static_cast<unsigned>(tile) % St::NUMBER;
-        good &= ~(1u << place);
         if (!of_nodes && block_of(a, min(at0 + SK, cached) - 1) >= base + filled) fill_table(block_of(a, at0));
         const unsigned to = lds0 + place * St::BYTES + wave * St::LOADS * 1024;
-        if (WHOLE && in_pages && !of_nodes && at0 + SK <= cached) {
-            // lane i: the first row of instruction i; and the stage's page i, all of which have to exist
-            const int at = at0 + wave * St::MINE + min(lane, St::LOADS - 1) * St::PER_LOAD, block = block_of(a, at), block0 = block_of(a, at0);
-            const int entry = table_s[block - base], any = table_s[min(block0 + lane, block_of(a, at0 + SK - 1)) - base];
-            const unsigned long long from = static_cast<unsigned long long>(static_cast<unsigned>(entry * a.page_size + at - block * a.page_size)) * a.page_pitch;
-            if (__all(static_cast<unsigned>(any) < static_cast<unsigned>(a.n_pages))) {
-                const int low = static_cast<int>(from), high = static_cast<int>(from >> 32);
-#pragma unroll
-                for (int i = 0; i < St::LOADS; ++i) {
-                    const size_t row = static_cast<size_t>(static_cast<unsigned>(__builtin_amdgcn_readlane(high, i))) << 32 | static_cast<unsigned>(__builtin_amdgcn_readlane(low, i));
-                    load_to_lds(reinterpret_cast<const unsigned char*>(a.k_pages) + head + row, offset[i], to + 1024 * i);
-                    load_to_lds(reinterpret_cast<const unsigned char*>(a.v_pages) + head + row, offset[i], to + St::MATRIX + 1024 * i);
-                }
-                if (lane == 0) valid_s[place][wave] = ALL_MINE;
-                good |= 1u << place;
-                return;
+        const bool whole = WHOLE && in_pages && !of_nodes && at0 + SK <= cached && all_pages;
+        good = (good & ~(1u << place)) | (whole ? 1u << place : 0u);
+        if (whole) {
+            if (tile - ready_from >= ready) {          // (of a stage behind the table's part some entry; it is found again when that part is there)
+                ready = AHEAD;
+                ready_from = tile;
+                const int at = at0 + lane / St::LOADS * SK + wave * St::MINE + lane % St::LOADS * St::PER_LOAD, block = min(block_of(a, at), base + filled - 1);
+                row_at = static_cast<unsigned long long>(static_cast<unsigned>(table_s[block - base] * a.page_size + at - block * a.page_size)) * a.page_pitch;
             }
+            const int from = (tile - ready_from) * St::LOADS, low = static_cast<int>(row_at), high = static_cast<int>(row_at >> 32);
+#pragma unroll
+            for (int i = 0; i < St::LOADS; ++i) {
+                const size_t row = static_cast<size_t>(static_cast<unsigned>(__builtin_amdgcn_readlane(high, from + i))) << 32 |
+                                   static_cast<unsigned>(__builtin_amdgcn_readlane(low, from + i));
+                load_to_lds(reinterpret_cast<const unsigned char*>(a.k_pages) + head + row, offset[i], to + 1024 * i);
+                load_to_lds(reinterpret_cast<const unsigned char*>(a.v_pages) + head + row, offset[i], to + St::MATRIX + 1024 * i);
+            }
+            if (lane == 0) valid_s[place][wave] = ALL_MINE;
+            return;
         }
         auto row_of = [&](int k, bool& there) {
             if (of_nodes) {
@@ -586,7 +616,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             }
             some = static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(some >> 32)))) << 32 |
                    static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(some)));
-            r.take_some(p, a, of_nodes, at0 + k0, some, first, nodes, [&](int j, int x) {
+            r.take_some(p, v, a, of_nodes, at0 + k0, some, first, nodes, [&](int j, int x) {
                 return *reinterpret_cast<const uint32_t*>(keys + value_at[j % 4][x] + j / 4 * 16 * St::ROW + 4 * (x % S::block_words(x)));
             });
         }
@@ -638,16 +668,15 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     for (int item = threadIdx.x; item < count * quads; item += NW * 64) {
         const int row = item / quads, d = (item - row * quads) * 4;
         const int at = row / (16 * RT) * KG * 16 * RT + row % (16 * RT);        // in the first key group's state; the others' lie 16 RT rows apart
-        float top = -INFINITY, sum = 0.f;
+        float top = LEAST_SCORE, sum = 0.f;
 #pragma unroll
         for (int i = 0; i < KG; ++i) top = fmaxf(top, ml_s[at + i * 16 * RT].x);
-        const float against = top == -INFINITY ? 0.f : top;
         f32x4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < KG; ++i) {
             const float2 ml = ml_s[at + i * 16 * RT];
             const f32x4 part = *reinterpret_cast<const f32x4*>(state_s + (at + i * 16 * RT) * PITCH + d);
-            const float weight = exp2_for<T>(ml.x - against);
+            const float weight = exp2_for<T>(ml.x - top);
             if (ml.y == 0.f) continue;          // (a key group whose keys nobody saw)
             sum += weight * ml.y;
 #pragma unroll
@@ -678,14 +707,13 @@ __global__ void __launch_bounds__(256) tree_attention_join_kernel(TreeAttentionP
     for (int item = blockIdx.z * 256 + threadIdx.x; item < a.n_heads * quads; item += gridDim.z * 256) {
         const int h = item / quads, d = (item - h * quads) * 4;
         const size_t pair = (static_cast<size_t>(t) * a.n_heads + h) * a.nsplit;
-        float top = -INFINITY, sum = 0.f;
+        float top = LEAST_SCORE, sum = 0.f;
         for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, state[2 * (pair + s)]);
-        const float against = top == -INFINITY ? 0.f : top;
         f32x4 v{0.f, 0.f, 0.f, 0.f};
         for (int s = 0; s < a.nsplit; ++s) {
             const float2 ml = *reinterpret_cast<const float2*>(state + 2 * (pair + s));
             const f32x4 part = *reinterpret_cast<const f32x4*>(a.ws + (pair + s) * a.head_dim + d);
-            const float weight = exp2_for<T>(ml.x - against);
+            const float weight = exp2_for<T>(ml.x - top);
             if (ml.y == 0.f) continue;
             sum += weight * ml.y;
 #pragma unroll
@@ -714,7 +742,7 @@ Plan plan_of(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_new,
     p.rt = 1;
     int row_groups = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8;
     if (p.nt <= (f32 ? 2 : 4) && rows > 64) { p.rt = 2; row_groups = rows <= 128 ? 4 : 8; }
-    if (p.nt == 8) row_groups = std::min(row_groups, 4);        // (registers)
+    if (p.nt > 4) row_groups = std::min(row_groups, 4);         // (registers)
     p.key_groups = std::min(p.nt <= 2 ? 4 : p.nt <= 4 ? 2 : 1, 8 / row_groups);
     p.waves = row_groups * p.key_groups;
     const int each = 16 * p.rt * row_groups;
@@ -751,7 +779,6 @@ int dispatch(const TreeAttentionParams& p, const Plan& plan, hipStream_t stream)
 #define TREE_MIDDLE(N) TREE_CASE(N, 1, ONE, 2, 2) TREE_CASE(N, 1, ONE, 4, 2) TREE_CASE(N, 1, ONE, 8, 2)
 #define TREE_WIDE(N) TREE_CASE(N, 1, ONE, 1, 1) TREE_CASE(N, 1, ONE, 2, 1) TREE_CASE(N, 1, ONE, 4, 1)
     TREE_NARROW(1) TREE_NARROW(2) TREE_MIDDLE(3) TREE_MIDDLE(4) TREE_WIDE(6) TREE_WIDE(8)
-    TREE_CASE(6, 1, ONE, 8, 1)
     if constexpr (sizeof(T) == 2) {
         TREE_CASE(3, 2, ONE, 8, 2) TREE_CASE(3, 2, ONE, 8, 1) TREE_CASE(4, 2, ONE, 8, 2) TREE_CASE(4, 2, ONE, 8, 1)
     } else {
