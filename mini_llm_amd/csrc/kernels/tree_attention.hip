@@ -325,15 +325,15 @@ struct Rows {
             for (int w = 0; w < CH; ++w) each |= not_finite(v[j][w], T{});
             odd |= each & exists(j);
         }
-        const bool special = __any(odd != 0);
-        weigh<true>(
-            [&](int j, int w) {
-                uint32_t x = v[j][w] & exists(j);
-                return special ? sifted(x, 0, T{}) : x;
-            },
-            weight, add, [&](int rt, auto&& product) { sum[rt] = product(sum[rt]); });
-        if (!special) return;
+        auto added = [&](int rt, auto&& product) { sum[rt] = product(sum[rt]); };
+        int plain = !__any(odd != 0);
+        asm volatile("" : "+v"(plain));          // (a lane's register, as where this function is called)
+        if (plain) {
+            weigh<true>([&](int j, int w) { return v[j][w] & exists(j); }, weight, add, added);
+            return;
+        }
         auto word = [&](int j, int w) { return stored(j, w) & exists(j); };
+        weigh<true>([&](int j, int w) { return sifted(word(j, w), 0, T{}); }, weight, add, added);
 #pragma unroll 1
         for (int kind = 1; kind <= 3; ++kind) {
             const float value = kind == 1 ? __builtin_nanf("") : kind == 2 ? INFINITY : -INFINITY;
@@ -534,8 +534,6 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     };
     auto place_of = [&](int k, int piece) { return 16 * (POW2 ? piece ^ (k & TURN) : (piece + k % 16) % PIECES); };
 
-    for (int i = 0; i < St::NUMBER - 1; ++i)
-        if (begin + i < end) ask(begin + i);
     // One loop over the wavefront's tiles of all stages: in two loops, one in the other, the outputs would be copied from the one's registers
     // to the other's for every tile. (A wavefront whose rows lie behind the last works on the last again, and writes nothing.)
     constexpr int TURNS = SK / KEYS / KG;
@@ -563,6 +561,10 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             for (int c = 0; c < CH; ++c) k[kt][c] = *reinterpret_cast<const uint4*>(keys + key_at[c] + kt * 16 * St::ROW);
     };
     const int steps = (end - begin) * TURNS;
+    // (not unrolled: code that runs once waits for its instructions to come)
+#pragma unroll 1
+    for (int i = 0; i < St::NUMBER - 1; ++i)
+        if (begin + i < end) ask(begin + i);
     if (steps > 0) {
         wait_tiles_and_meet<St::NUMBER - 3, 2 * St::LOADS>(min(St::NUMBER - 3, end - 1 - begin));
         read_keys(0);
