@@ -424,14 +424,13 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     const int first = w.first, nodes = w.nodes, hk = w.hk, cached = w.cached;
     const int* table = a.block_tables + static_cast<size_t>(w.b) * a.max_blocks;
 
-    // A part of the block table lies in LDS, from entry `base` on; all of the workgroup meet here. Whether all of its entries that the cache
-    // reaches name pages is known then.
-    int base = 0, filled = 0, all_pages = 0, ready = 0, ready_from = 0;
+    // A part of the block table lies in LDS, from entry `base` on; all of the workgroup meet here. Returns whether all of its entries that the
+    // cache reaches name pages.
+    int base = 0, filled = 0;
     auto fill_table = [&](int from) {
         lds_barrier();
         base = from;
         filled = min(TABLE_ENTRIES, a.max_blocks - from);
-        ready = 0;
         const int reached = min(filled, block_of(a, cached - 1) + 1 - from);
         int good = 1;
         for (int i = threadIdx.x; i < filled; i += NW * 64) {
@@ -439,7 +438,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             table_s[i] = entry;
             good &= i >= reached || static_cast<unsigned>(entry) < static_cast<unsigned>(a.n_pages);
         }
-        all_pages = __syncthreads_and(good);
+        return __syncthreads_and(good) != 0;
     };
     // Tiles of SK keys: those of the cache from the window's first on, then the nodes'. A split has `per` neighbouring ones.
     int first_tile = 0;
@@ -460,50 +459,55 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     // would have it wait in the loop, every time, for all that is on its way.
     R r;
     r.begin(a, first, w.rows, w.group, hk, row0, row_bytes);
-    if (begin < cache_tiles) fill_table(min(block_of(a, (begin + first_tile) * SK), a.max_blocks - 1));
+    // Tiles below whole_end have SK keys that exist, and load instructions that take whole rows of one page each.
+    constexpr bool WHOLE = St::PER_LOAD > 0 && 64 % PIECES == 0 && POW2;
+    int whole_end = WHOLE && a.page_size % std::max(St::PER_LOAD, 1) == 0 ? cached / SK - first_tile : 0;
+    if (begin < cache_tiles && !fill_table(min(block_of(a, (begin + first_tile) * SK), a.max_blocks - 1))) whole_end = min(whole_end, begin);
     r.wait_for_queries(row_bytes, a.negative);
 
     const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)stage_s));
     const size_t head = static_cast<size_t>(hk) * row_bytes;
-    // Asks for a stage. (All of the workgroup come here, behind a barrier after which nobody reads what it fills.) A wavefront has MINE
-    // neighbouring rows of it. Where each of its load instructions takes whole rows that lie in one page, and all of them exist, an instruction's
-    // address is the page's and an offset that the lane keeps: a few scalar instructions a load. Otherwise every lane finds its row.
-    constexpr bool WHOLE = St::PER_LOAD > 0 && 64 % PIECES == 0 && POW2;
+    // Asks for stage after stage. (All of the workgroup come here, behind a barrier after which nobody reads what it fills.) A wavefront has MINE
+    // neighbouring rows of it. Of tiles below whole_end an instruction's address is its first row's and an offset that the lane keeps, and the
+    // rows are found AHEAD tiles at a time, from tile ready_from on: lane s * LOADS + i has instruction i of tile ready_from + s. A few scalar
+    // instructions a load are left: between two barriers there is nothing else to do for a unit. Otherwise every lane finds its row.
     constexpr unsigned long long ALL_MINE = St::MINE == 64 ? ~0ull : (1ull << (St::MINE % 64)) - 1;
-    const bool in_pages = WHOLE && a.page_size % std::max(St::PER_LOAD, 1) == 0;
+    constexpr int AHEAD = 64 / St::LOADS;
     unsigned offset[St::LOADS];
 #pragma unroll
     for (int i = 0; i < St::LOADS; ++i) {
         const int k = wave * St::MINE + i * St::PER_LOAD + lane / PIECES, piece = (lane % PIECES) ^ (k & TURN);
         offset[i] = (lane / PIECES) * a.page_pitch + (16 * piece < row_bytes ? 16 * piece : 0);
     }
-    // Where the first rows of AHEAD stages' instructions lie, from stage ready_from on: lane s * LOADS + i has instruction i of stage s.
-    constexpr int AHEAD = 64 / St::LOADS;
+    const unsigned char *k_head = reinterpret_cast<const unsigned char*>(a.k_pages) + head, *v_head = reinterpret_cast<const unsigned char*>(a.v_pages) + head;
     unsigned long long row_at = 0;
-    unsigned good = 0;             // a bit a stage: all of its keys exist
+    int ready_from = 0, ready_end = 0, ask_place = 0;      // (tiles from ready_from to ready_end; the stage that is filled next)
     auto ask = [&](int tile) {
-        const bool of_nodes = tile >= cache_tiles;
-        const int at0 = (of_nodes ? tile - cache_tiles : tile + first_tile) * SK, place = static_cast<unsigned>(tile) % St::NUMBER;
-        if (!of_nodes && block_of(a, min(at0 + SK, cached) - 1) >= base + filled) fill_table(block_of(a, at0));
+        const int place = ask_place;
+        ask_place = place + 1 == St::NUMBER ? 0 : place + 1;
         const unsigned to = lds0 + place * St::BYTES + wave * St::LOADS * 1024;
-        const bool whole = WHOLE && in_pages && !of_nodes && at0 + SK <= cached && all_pages;
-        good = (good & ~(1u << place)) | (whole ? 1u << place : 0u);
-        if (whole) {
-            if (tile - ready_from >= ready) {          // (of a stage behind the table's part some entry; it is found again when that part is there)
-                ready = AHEAD;
-                ready_from = tile;
+        const bool of_nodes = tile >= cache_tiles;
+        const int at0 = (of_nodes ? tile - cache_tiles : tile + first_tile) * SK;
+        if (tile >= ready_end) {
+            if (!of_nodes && block_of(a, min(at0 + SK, cached) - 1) >= base + filled && !fill_table(block_of(a, at0))) whole_end = min(whole_end, tile);
+            if (tile < whole_end) {
+                // (of a tile behind the table's part some entry: it is found again when that part is there)
                 const int at = at0 + lane / St::LOADS * SK + wave * St::MINE + lane % St::LOADS * St::PER_LOAD, block = min(block_of(a, at), base + filled - 1);
                 row_at = static_cast<unsigned long long>(static_cast<unsigned>(table_s[block - base] * a.page_size + at - block * a.page_size)) * a.page_pitch;
+                const long long covered = (static_cast<long long>(base + filled) * a.page_size - at0) / SK;
+                ready_from = tile;
+                ready_end = min(tile + static_cast<int>(min(covered, static_cast<long long>(AHEAD))), whole_end);
             }
+        }
+        if (tile < ready_end) {
             const int from = (tile - ready_from) * St::LOADS, low = static_cast<int>(row_at), high = static_cast<int>(row_at >> 32);
 #pragma unroll
             for (int i = 0; i < St::LOADS; ++i) {
                 const size_t row = static_cast<size_t>(static_cast<unsigned>(__builtin_amdgcn_readlane(high, from + i))) << 32 |
                                    static_cast<unsigned>(__builtin_amdgcn_readlane(low, from + i));
-                load_to_lds(reinterpret_cast<const unsigned char*>(a.k_pages) + head + row, offset[i], to + 1024 * i);
-                load_to_lds(reinterpret_cast<const unsigned char*>(a.v_pages) + head + row, offset[i], to + St::MATRIX + 1024 * i);
+                load_to_lds(k_head + row, offset[i], to + 1024 * i);
+                load_to_lds(v_head + row, offset[i], to + St::MATRIX + 1024 * i);
             }
-            if (lane == 0) valid_s[place][wave] = ALL_MINE;
             return;
         }
         auto row_of = [&](int k, bool& there) {
@@ -550,11 +554,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             value_at[i][x] = St::MATRIX + row * St::ROW + place_of(row, byte / 16) + byte % 16;
         }
     uint4 k[KT][CH];
-    auto tile_of = [&](int step) {
-        return stage_s + static_cast<unsigned>(begin + step / TURNS) % St::NUMBER * St::BYTES + (step % TURNS * KG + kg) * (KEYS * St::ROW);
-    };
-    auto read_keys = [&](int step) {
-        const unsigned char* keys = tile_of(step);
+    auto read_keys = [&](const unsigned char* keys) {
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -567,12 +567,13 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
         if (begin + i < end) ask(begin + i);
     if (steps > 0) {
         wait_tiles_and_meet<St::NUMBER - 3, 2 * St::LOADS>(min(St::NUMBER - 3, end - 1 - begin));
-        read_keys(0);
+        read_keys(stage_s + kg * (KEYS * St::ROW));
     }
+    // (tiles from seen_begin to whole_end: every row sees all keys)
+    const int seen_begin = a.window > 0 ? (max(r.low_most, 0) + SK - 1) / SK - first_tile : 0;
+    int turn = 0, tile = begin, place = 0;
     for (int step = 0; step < steps; ++step) {
-        const int turn = step % TURNS, tile = begin + step / TURNS, place = static_cast<unsigned>(tile) % St::NUMBER;
-        const unsigned char* keys = tile_of(step);
-        const int k0 = (turn * KG + kg) * KEYS;
+        const unsigned char* keys = stage_s + place * St::BYTES + (turn * KG + kg) * (KEYS * St::ROW);
         if (turn == 0) {
             // the next stage has come (those behind it may be on their way), and all have read the one in front of this
             wait_tiles_and_meet<St::NUMBER - 3, 2 * St::LOADS>(max(0, min(St::NUMBER - 3, end - 2 - tile)));
@@ -598,23 +599,31 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
         float p[RT][4 * KT];
         r.scores(p, row_bytes, k);
         __builtin_amdgcn_sched_barrier(0);
-        read_keys(min(step + 1, steps - 1));
+        const int here = place, tile_here = tile, k0 = (turn * KG + kg) * KEYS;
+        if (++turn == TURNS) {
+            turn = 0;
+            ++tile;
+            place = place + 1 == St::NUMBER ? 0 : place + 1;
+        }
+        if (step + 1 < steps) read_keys(stage_s + place * St::BYTES + (turn * KG + kg) * (KEYS * St::ROW));
         __builtin_amdgcn_sched_barrier(0);
-        const bool of_nodes = tile >= cache_tiles;
-        const int at0 = (of_nodes ? tile - cache_tiles : tile + first_tile) * SK;
         // (The condition is kept in a lane's register: as a scalar branch, which the same one in all lanes could be, the compiler gives the outputs other
         // registers on either side of a product, and moves or spills them every time.)
-        int all_seen = (good >> place & 1) && (a.window <= 0 || at0 >= r.low_most);
+        int all_seen = tile_here >= seen_begin && tile_here < whole_end;
         asm volatile("" : "+v"(all_seen));
         if (all_seen) {
             r.take(p, a.scale, v);
         } else {
             unsigned long long some = 0;
-            if (St::MINE >= KEYS) {
-                some = valid_s[place][k0 / St::MINE] >> (k0 % St::MINE) & R::ALL;
+            const bool of_nodes = tile_here >= cache_tiles;
+            const int at0 = (of_nodes ? tile_here - cache_tiles : tile_here + first_tile) * SK;
+            if (tile_here < whole_end) {
+                some = R::ALL;
+            } else if (St::MINE >= KEYS) {
+                some = valid_s[here][k0 / St::MINE] >> (k0 % St::MINE) & R::ALL;
             } else {
 #pragma unroll
-                for (int i = 0; i < KEYS / St::MINE; ++i) some |= valid_s[place][k0 / St::MINE + i] << (i * St::MINE);
+                for (int i = 0; i < KEYS / St::MINE; ++i) some |= valid_s[here][k0 / St::MINE + i] << (i * St::MINE);
             }
             some = static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(some >> 32)))) << 32 |
                    static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(some)));
