@@ -644,6 +644,9 @@ def tree_max_nodes() -> int:
     return int(engine_library().mllm_op_tree_max_nodes())
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _here(*tensors: Optional[torch.Tensor]) -> int:
     """All on one GPU, and that the current one (whose current stream the op is launched on); its number."""
     devices = {t.get_device() for t in tensors if t is not None}
@@ -651,8 +654,8 @@ def _here(*tensors: Optional[torch.Tensor]) -> int:
         _gpu(*tensors)
         raise KernelError(f"tensors are on GPUs {sorted(devices)}")
     device = devices.pop()
-    if device != torch.cuda.current_device():
-        raise KernelError(f"tensors are on cuda:{device}, the current device is cuda:{torch.cuda.current_device()}")
+    if device != _current_device():
+        raise KernelError(f"tensors are on cuda:{device}, the current device is cuda:{_current_device()}")
     return device
 
 
@@ -660,21 +663,25 @@ def _stream_of(device: int) -> int:
     return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
+_INT32 = torch.int32
+
+
 def _counted(t: torch.Tensor, name: str, n: int) -> int:
     """The address of n whole numbers."""
-    if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+    if t.dtype is not _INT32 or t.shape != (n,) or not t.is_contiguous():
         raise KernelError(f"{name} must be contiguous int32 [{n}], got {tuple(t.shape)} {t.dtype}")
     return t.data_ptr()
 
 
 def _matrix(t: torch.Tensor, name: str) -> tuple:
     """The numbers of a Tensor2."""
-    if t.dim() == 2:
+    try:
         rows, cols = t.shape
         across, along = t.stride()
-        dtype = _DT.get(t.dtype)
-        if dtype is not None and along == 1 and (rows > 1 or across >= cols):
-            return t.data_ptr(), dtype, rows, cols, across
+        if along == 1 and (rows > 1 or across >= cols):
+            return t.data_ptr(), _DT[t.dtype], rows, cols, across
+    except (ValueError, KeyError):
+        pass
     c = t2(t, name)
     return c.data or 0, c.dtype, c.rows, c.cols, c.stride
 
@@ -757,7 +764,8 @@ def step_maps(maps: StepMaps, rows: Optional[torch.Tensor], n_new: torch.Tensor,
     device = _here(rows, n_new, lengths, pages, parents, maps.cu_q)
     a = _bytes(_MAPS_BYTES, at_rows, at_new, at_lengths, pages.data_ptr(), at_parents, pages.stride(0) if requests > 1 else cols, B, requests, T, page_size,
                n_pages, blocks, maps.max_new, words, *mine)
-    _ok(engine_library().mllm_op_step_maps(a, _stream_of(device)))
+    if engine_library().mllm_op_step_maps(a, _stream_of(device)):
+        _ok(1)
     return maps
 
 
@@ -840,7 +848,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, n_heads: i
     T, B = q.shape[0], cached.numel()
     at_tables, blocks = _whole_table(block_tables, "block_tables", B)
     at_cached, at_cu, at_positions = _counted(cached, "cached", B), _counted(cu_q, "cu_q", B + 1), 0
-    if ancestors.dim() != 2 or ancestors.dtype is not torch.int64 or not ancestors.is_contiguous() or ancestors.shape[0] != T:
+    words = ancestors.shape[-1] if ancestors.dim() else 0
+    if ancestors.dtype is not torch.int64 or ancestors.shape != (T, words) or not ancestors.is_contiguous():
         raise KernelError(f"ancestors must be contiguous int64 [{T}, words]")
     if positions is not None:
         at_positions = _counted(positions, "positions", T)
@@ -849,21 +858,16 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, n_heads: i
     mq, mk, mv, mkp, mvp, mo = _matrix(q, "q"), _matrix(k, "k"), _matrix(v, "v"), _matrix(k_pages, "k_pages"), _matrix(v_pages, "v_pages"), _matrix(out, "out")
     device = _here(q, k, v, k_pages, v_pages, block_tables, cached, cu_q, ancestors, positions, out)
 
-    def numbers(workspace, floats):
-        return _bytes(_ATTENTION_BYTES, *mq, *mk, *mv, n_heads, n_kv_heads, head_dim, *mkp, *mvp, page_size, at_tables, B, blocks, at_cached, at_cu, ancestors.data_ptr(),
-                      ancestors.shape[1], at_positions, scale, window, max_new, max_cached, *mo, workspace, floats)
-
-    lib = engine_library()
     try:
         floats = _tree_workspace(T, B, n_heads, n_kv_heads, head_dim, max_new, max_cached, window, mq[1])
     except ctypes.ArgumentError:
         raise KernelError("tree_attention: sizes are whole numbers of 32 bits") from None
-    if floats > 0:
-        # (of the caller's stream and, in a capture, of the graph's own pool: two graphs share none)
-        ws = torch.empty(floats, dtype=torch.float32, device=q.device)
-        _ok(lib.mllm_op_tree_attention(numbers(ws.data_ptr(), floats), _stream_of(device)))
-    else:
-        _ok(lib.mllm_op_tree_attention(numbers(0, 0), _stream_of(device)))
+    # (of the caller's stream and, in a capture, of the graph's own pool: two graphs share none)
+    ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats > 0 else None
+    a = _bytes(_ATTENTION_BYTES, *mq, *mk, *mv, n_heads, n_kv_heads, head_dim, *mkp, *mvp, page_size, at_tables, B, blocks, at_cached, at_cu, ancestors.data_ptr(), words,
+               at_positions, scale, window, max_new, max_cached, *mo, 0 if ws is None else ws.data_ptr(), floats)
+    if engine_library().mllm_op_tree_attention(a, _stream_of(device)):
+        _ok(1)
     return out
 
 
@@ -895,4 +899,5 @@ def tree_accept(choices: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor,
     device = _here(choices, ids, parents, cu_q, cached, block_tables, kept, path, next_token, slots, lengths, rows)
     a = _bytes(_ACCEPT_BYTES, tokens[0], tokens[1], tokens[2], at_cu, at_cached, at_tables, at_rows, B, T, page_size, n_pages, blocks, max_new, requests, at_kept, at_path,
                at_next, tokens[3], at_lengths)
-    _ok(engine_library().mllm_op_tree_accept(a, _stream_of(device)))
+    if engine_library().mllm_op_tree_accept(a, _stream_of(device)):
+        _ok(1)
