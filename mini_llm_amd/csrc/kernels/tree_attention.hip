@@ -50,7 +50,8 @@ struct TreeAttentionParams {
     float* ws;
 };
 
-// Sizes of a kernel for heads of more than 32 (NT - 1), up to 32 NT columns (less for the NT that stand for two).
+// Sizes of a kernel for heads of more than 16 NT, up to 32 NT columns (NT = 1: from the first). A row has a power of two of columns in LDS, so that
+// whole rows fill a load instruction; narrower heads leave some of them unused (96 columns as 128: 1.5 times as fast as rows packed without a gap).
 template <typename T, int NT, int KEY_GROUPS_OF_16>
 struct Shape {
     static constexpr int KT = KEY_GROUPS_OF_16;            // 16-key groups of a tile (bfloat16: a product step of values takes two)
@@ -58,10 +59,9 @@ struct Shape {
     static constexpr int CH = NT * sizeof(T) / 2;          // 64-byte pieces of a row; words of a value row in a lane
     static constexpr int PER = 4 / sizeof(T);              // elements of a word
     static constexpr int TILES = 2 * NT;                   // 16-column tiles of the output
-    static constexpr int LEAST = NT == 6 ? 4 : NT == 8 ? 6 : NT - 1;       // heads are wider than 32 LEAST
-    // of word w: the first word of its block (of 4, 2 or 1 words a lane) and the block's words
-    static constexpr int block_words(int w) { return w < CH / 4 * 4 ? 4 : w < CH / 2 * 2 ? 2 : 1; }
-    static constexpr int block_first(int w) { return w / block_words(w) * block_words(w); }
+    static constexpr int LEAST = NT / 2;                   // heads are wider than 32 LEAST
+    static_assert((NT & (NT - 1)) == 0, "a power of two");
+    static constexpr int BLOCK = std::min(CH, 4);          // words of a lane that lie together
 };
 
 // Ones (1 in the lowest bit of each element) where a word's elements are not finite. In whole-number arithmetic on all elements of the word at
@@ -347,11 +347,9 @@ struct Rows {
         }
     }
 
-    // Where o[x][rt][i] stands in its row: column() + E(x) * (4 G + i), E elements a lane has in the block.
-    __device__ __forceinline__ static constexpr int each(int x) { return S::block_words(x / S::PER) * S::PER; }
-    __device__ __forceinline__ static constexpr int column(int x) {
-        return S::block_first(x / S::PER) * 16 * S::PER + (x / S::PER - S::block_first(x / S::PER)) * S::PER + x % S::PER;
-    }
+    // o[x][rt][i] stands in column column(x) + EACH (4 G + i) of its row: EACH elements a lane has in a block.
+    static constexpr int EACH = S::BLOCK * S::PER;
+    __device__ __forceinline__ static constexpr int column(int x) { return x / EACH * 16 * EACH + x % EACH; }
 };
 
 // What a workgroup works on, the same in all its threads.
@@ -383,8 +381,7 @@ __device__ __forceinline__ float2* split_state(const TreeAttentionParams& a, siz
     return reinterpret_cast<float2*>(a.ws + static_cast<size_t>(a.tokens) * a.n_heads * a.nsplit * a.head_dim) + pair;
 }
 
-// 16-byte piece p of row k of a stage lies at piece p ^ (k % 16) (rotated by it where a row's pieces are no power of two), so that 16 lanes that
-// read one piece of 16 rows meet no bank twice.
+// 16-byte piece p of row k of a stage lies at piece p ^ (k % 16), so that 16 lanes that read one piece of 16 rows meet no bank twice.
 constexpr int TABLE_ENTRIES = 2048;
 template <typename T, int NT, int K16, int NW, int KG>
 struct Stage {
@@ -400,7 +397,7 @@ struct Stage {
     static constexpr int NUMBER = 4 * BYTES <= 131072 ? 4 : 3;            // one is read, the next has come, the others are on their way
     static constexpr int LOADS = KEYS * PIECES / 64 / NW;                 // of a wavefront, a stage and matrix
     static_assert(LOADS * 64 * NW == KEYS * PIECES, "whole instructions");
-    static constexpr int MINE = KEYS / NW, PER_LOAD = 64 / PIECES;        // rows of a wavefront (it loads these), rows of a load instruction (0: less than one)
+    static constexpr int MINE = KEYS / NW, PER_LOAD = 64 / PIECES;        // rows of a wavefront (it loads these), rows of a load instruction
     static_assert(MINE <= 64 && KEYS % NW == 0, "a bit a row");
 };
 
@@ -410,7 +407,6 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     using S = Shape<T, NT, K16>;
     using St = Stage<T, NT, K16, NW, KG>;
     constexpr int KT = S::KT, KEYS = S::KEYS, CH = S::CH, TILES = S::TILES, PIECES = St::PIECES, SK = St::KEYS, RG = NW / KG, PITCH = 32 * NT + 4;
-    constexpr bool POW2 = (PIECES & (PIECES - 1)) == 0;
     constexpr int TURN = std::min(PIECES, 16) - 1;
     // the stages [keys, values][SK][PIECES * 16]; at the end the states [wavefront][16 RT][PITCH], then their maxima and sums
     extern __shared__ __attribute__((aligned(16))) unsigned char stage_s[];
@@ -460,8 +456,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     R r;
     r.begin(a, first, w.rows, w.group, hk, row0, row_bytes);
     // Tiles below whole_end have SK keys that exist, and load instructions that take whole rows of one page each.
-    constexpr bool WHOLE = St::PER_LOAD > 0 && 64 % PIECES == 0 && POW2;
-    int whole_end = WHOLE && a.page_size % std::max(St::PER_LOAD, 1) == 0 ? cached / SK - first_tile : 0;
+    int whole_end = a.page_size % St::PER_LOAD == 0 ? cached / SK - first_tile : 0;
     if (begin < cache_tiles && !fill_table(min(block_of(a, (begin + first_tile) * SK), a.max_blocks - 1))) whole_end = min(whole_end, begin);
     r.wait_for_queries(row_bytes, a.negative);
 
@@ -470,7 +465,8 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     // Asks for stage after stage. (All of the workgroup come here, behind a barrier after which nobody reads what it fills.) A wavefront has MINE
     // neighbouring rows of it. Of tiles below whole_end an instruction's address is its first row's and an offset that the lane keeps, and the
     // rows are found AHEAD tiles at a time, from tile ready_from on: lane s * LOADS + i has instruction i of tile ready_from + s. A few scalar
-    // instructions a load are left: between two barriers there is nothing else to do for a unit. Otherwise every lane finds its row.
+    // instructions a load are left: between two barriers there is nothing else to do for a unit. Otherwise a lane finds a row, and hands it to those
+    // that load it.
     constexpr unsigned long long ALL_MINE = St::MINE == 64 ? ~0ull : (1ull << (St::MINE % 64)) - 1;
     constexpr int AHEAD = 64 / St::LOADS;
     unsigned offset[St::LOADS];
@@ -510,17 +506,17 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             }
             return;
         }
-        auto row_of = [&](int k, bool& there) {
-            if (of_nodes) {
-                there = at0 + k < nodes;
-                return first + min(at0 + k, nodes - 1);
-            }
-            const int at = min(at0 + k, cached - 1), block = block_of(a, at), entry = table_s[block - base];
-            there = at0 + k < cached && static_cast<unsigned>(entry) < static_cast<unsigned>(a.n_pages);
-            return there ? entry * a.page_size + at - block * a.page_size : 0;
-        };
+        const int mine = at0 + wave * St::MINE + lane % St::MINE;
         bool there;
-        row_of(wave * St::MINE + lane % St::MINE, there);
+        int row;
+        if (of_nodes) {
+            there = mine < nodes;
+            row = first + min(mine, nodes - 1);
+        } else {
+            const int at = min(mine, cached - 1), block = block_of(a, at), entry = table_s[block - base];
+            there = mine < cached && static_cast<unsigned>(entry) < static_cast<unsigned>(a.n_pages);
+            row = there ? entry * a.page_size + at - block * a.page_size : 0;
+        }
         const unsigned long long bits = __ballot(there) & ALL_MINE;
         if (lane == 0) valid_s[place][wave] = bits;
         const unsigned char* kb = reinterpret_cast<const unsigned char*>(of_nodes ? a.k : a.k_pages) + head;
@@ -528,15 +524,14 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
         const size_t k_pitch = of_nodes ? a.ldk : a.page_pitch, v_pitch = of_nodes ? a.ldv : a.page_pitch;
 #pragma unroll 1
         for (int i = 0; i < St::LOADS; ++i) {
-            const int slot = (wave * St::LOADS + i) * 64 + lane, k = slot / PIECES, put = slot % PIECES;
-            const int piece = POW2 ? put ^ (k & TURN) : (put + PIECES - k % 16 % PIECES) % PIECES;
+            const int k = i * St::PER_LOAD + lane / PIECES, piece = lane % PIECES ^ ((wave * St::MINE + k) & TURN);
             const int off = 16 * piece < row_bytes ? 16 * piece : 0;
-            const size_t row = row_of(k, there);
-            load_to_lds(kb, row * k_pitch + off, to + 1024 * i);
-            load_to_lds(vb, row * v_pitch + off, to + St::MATRIX + 1024 * i);
+            const size_t from = __shfl(row, k, 64);
+            load_to_lds(kb, from * k_pitch + off, to + 1024 * i);
+            load_to_lds(vb, from * v_pitch + off, to + St::MATRIX + 1024 * i);
         }
     };
-    auto place_of = [&](int k, int piece) { return 16 * (POW2 ? piece ^ (k & TURN) : (piece + k % 16) % PIECES); };
+    auto place_of = [&](int k, int piece) { return 16 * (piece ^ (k & TURN)); };
 
     // One loop over the wavefront's tiles of all stages: in two loops, one in the other, the outputs would be copied from the one's registers
     // to the other's for every tile. (A wavefront whose rows lie behind the last works on the last again, and writes nothing.)
@@ -550,7 +545,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int x = 0; x < CH; ++x) {
-            const int row = 4 * G + i, n = S::block_words(x), byte = 64 * S::block_first(x) + 4 * n * c16;
+            const int row = 4 * G + i, byte = 64 * (x / S::BLOCK * S::BLOCK) + 4 * S::BLOCK * c16;
             value_at[i][x] = St::MATRIX + row * St::ROW + place_of(row, byte / 16) + byte % 16;
         }
     uint4 k[KT][CH];
@@ -583,12 +578,12 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
 #pragma unroll
         for (int j = 0; j < 4 * KT; ++j)
 #pragma unroll
-            for (int x = 0; x < CH; x += S::block_words(x)) {
+            for (int x = 0; x < CH; x += S::BLOCK) {
                 const unsigned char* at = keys + value_at[j % 4][x] + j / 4 * 16 * St::ROW;
-                if (S::block_words(x) == 4) {
+                if (S::BLOCK == 4) {
                     const uint4 u = *reinterpret_cast<const uint4*>(at);
                     v[j][x] = u.x; v[j][x + 1] = u.y; v[j][x + 2] = u.z; v[j][x + 3] = u.w;
-                } else if (S::block_words(x) == 2) {
+                } else if (S::BLOCK == 2) {
                     const uint2 u = *reinterpret_cast<const uint2*>(at);
                     v[j][x] = u.x; v[j][x + 1] = u.y;
                 } else {
@@ -628,7 +623,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             some = static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(some >> 32)))) << 32 |
                    static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(some)));
             r.take_some(p, v, a, of_nodes, at0 + k0, some, first, nodes, [&](int j, int x) {
-                return *reinterpret_cast<const uint32_t*>(keys + value_at[j % 4][x] + j / 4 * 16 * St::ROW + 4 * (x % S::block_words(x)));
+                return *reinterpret_cast<const uint32_t*>(keys + value_at[j % 4][x] + j / 4 * 16 * St::ROW + 4 * (x % S::BLOCK));
             });
         }
     }
@@ -645,13 +640,13 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             const size_t pair = (static_cast<size_t>(t) * a.n_heads + h) * a.nsplit + w.split;
             float* part = a.ws + pair * a.head_dim;
 #pragma unroll
-            for (int x = 0; x < TILES; x += R::each(x))
+            for (int x = 0; x < TILES; x += R::EACH)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int d = R::column(x) + R::each(x) * (4 * G + i);
+                    const int d = R::column(x) + R::EACH * (4 * G + i);
                     if (d >= a.head_dim) continue;
 #pragma unroll
-                    for (int e = 0; e < R::each(x); ++e) {
+                    for (int e = 0; e < R::EACH; ++e) {
                         if (a.nsplit == 1) to[d + e] = from_float<T>(r.o[x + e][rt][i] * inv);
                         else part[d + e] = r.o[x + e][rt][i];
                     }
@@ -672,7 +667,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
 #pragma unroll
         for (int x = 0; x < TILES; ++x)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) to[R::column(x) + R::each(x) * (4 * G + i)] = r.o[x][rt][i];
+            for (int i = 0; i < 4; ++i) to[R::column(x) + R::EACH * (4 * G + i)] = r.o[x][rt][i];
     }
     lds_barrier();
     const int quads = a.head_dim / 4, count = min(16 * RT * RG, w.rows - group0);
@@ -745,9 +740,7 @@ struct Plan {
 Plan plan_of(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_new, int max_cached, int window, int dtype) {
     Plan p;
     const bool f32 = dtype == MLLM_F32;
-    p.nt = (head_dim + 31) / 32;
-    if (p.nt == 5) p.nt = 6;
-    if (p.nt == 7) p.nt = 8;
+    p.nt = head_dim <= 32 ? 1 : head_dim <= 64 ? 2 : head_dim <= 128 ? 4 : 8;
     const long long rows = static_cast<long long>(max_new) * (n_heads / n_kv_heads);
     // Key groups: as many as there is a 32-KB stage for (at most 8 wavefronts).
     p.rt = 1;
@@ -789,11 +782,11 @@ int dispatch(const TreeAttentionParams& p, const Plan& plan, hipStream_t stream)
 #define TREE_NARROW(N) TREE_CASE(N, 1, ONE, 4, 4) TREE_CASE(N, 1, ONE, 8, 4) TREE_CASE(N, 1, TWO, 8, 2) TREE_CASE(N, 2, ONE, 8, 2) TREE_CASE(N, 2, ONE, 8, 1)
 #define TREE_MIDDLE(N) TREE_CASE(N, 1, ONE, 2, 2) TREE_CASE(N, 1, ONE, 4, 2) TREE_CASE(N, 1, ONE, 8, 2)
 #define TREE_WIDE(N) TREE_CASE(N, 1, ONE, 1, 1) TREE_CASE(N, 1, ONE, 2, 1) TREE_CASE(N, 1, ONE, 4, 1)
-    TREE_NARROW(1) TREE_NARROW(2) TREE_MIDDLE(3) TREE_MIDDLE(4) TREE_WIDE(6) TREE_WIDE(8)
+    TREE_NARROW(1) TREE_NARROW(2) TREE_MIDDLE(4) TREE_WIDE(8)
     if constexpr (sizeof(T) == 2) {
-        TREE_CASE(3, 2, ONE, 8, 2) TREE_CASE(3, 2, ONE, 8, 1) TREE_CASE(4, 2, ONE, 8, 2) TREE_CASE(4, 2, ONE, 8, 1)
+        TREE_CASE(4, 2, ONE, 8, 2) TREE_CASE(4, 2, ONE, 8, 1)
     } else {
-        TREE_CASE(3, 1, ONE, 8, 1) TREE_CASE(4, 1, ONE, 8, 1)
+        TREE_CASE(4, 1, ONE, 8, 1)
     }
 #undef TREE_WIDE
 #undef TREE_MIDDLE
