@@ -56,10 +56,14 @@ __global__ void __launch_bounds__(TREE_THREADS) step_maps_kernel(StepMapsParams 
         return static_cast<unsigned>(r) < static_cast<unsigned>(a.n_requests) ? r : -1;
     };
     auto count_of = [&](int i) { return row_of(i) < 0 ? 0 : min(max(a.n_new[i], 0), a.max_new); };
+    // (what does not need the place of the first token is read while the counts come)
+    const bool behind = b == a.n_seqs;
+    const int row = behind ? -1 : row_of(b), count = behind ? 0 : count_of(b);
+    const int cached = row < 0 ? 0 : min(max(a.lengths[row], 0), INT32_MAX - a.max_new);
     int before = 0;
     for (int i = tid; i < b; i += TREE_THREADS) before += count_of(i);
     const int first = min(block_sum_int(before, sums), a.tokens);
-    if (b == a.n_seqs) {
+    if (behind) {
         for (int t = first + part * TREE_THREADS + tid; t < a.tokens; t += parts * TREE_THREADS) {
             a.token_seq[t] = 0;
             a.positions[t] = 0;
@@ -69,8 +73,7 @@ __global__ void __launch_bounds__(TREE_THREADS) step_maps_kernel(StepMapsParams 
         if (part == 0 && tid == 0) a.cu_q[b] = first;
         return;
     }
-    const int row = row_of(b), n = min(count_of(b), a.tokens - first);
-    const int cached = row < 0 ? 0 : min(max(a.lengths[row], 0), INT32_MAX - a.max_new);
+    const int n = min(count, a.tokens - first);
     const int* list = a.pages + static_cast<size_t>(max(row, 0)) * a.ld_pages;
     if (part == 0 && tid == 0) {
         a.cu_q[b] = first;
@@ -202,8 +205,8 @@ int mllm_step_maps(const int* rows, const int* n_new, const int* lengths, const 
     if (parents != nullptr && (max_new > TREE_MAX_NODES || words < (max_new + 63) / 64 || words > TREE_MAX_NODES / 64)) return -1;
     const StepMapsParams p{rows, n_new, lengths, pages, parents, ld_pages, n_seqs, n_requests, tokens, page_size, n_pages, max_blocks, max_new,
                            parents != nullptr ? words : 0, cu_q, cached, ctx_len, token_seq, positions, slots, block_tables, ancestors};
-    // (a workgroup for every 2,048 entries of a table or tokens of a portion)
-    const int parts = std::min(64, (std::max(max_blocks, parents != nullptr ? 1 : max_new) + 2047) / 2048);
+    // (a workgroup for every 1,024 entries of a table or tokens of a portion)
+    const int parts = std::min(64, (std::max(max_blocks, parents != nullptr ? 1 : max_new) + 1023) / 1024);
     step_maps_kernel<<<dim3(n_seqs + 1, parts), TREE_THREADS, 0, stream>>>(p);
     MLLM_LAUNCH_CHECK();
     return 0;
