@@ -60,8 +60,8 @@ __global__ void __launch_bounds__(ROT_THREADS)
 rotary_kernel(const T* x, T* out, const int* __restrict__ positions, const unsigned long long* __restrict__ turns, int tokens, int pairs, int n_heads,
               int head_dim, long long ldx, long long ldo, int places, int heads_each, float amplitude) {
     const long long item = static_cast<long long>(blockIdx.x) * ROT_THREADS + threadIdx.x;
+    if (item / places >= tokens) return;
     const int t = static_cast<int>(item / places), place = static_cast<int>(item % places);
-    if (t >= tokens) return;
     const int position = positions[t], h0 = blockIdx.y * heads_each, h1 = min(h0 + heads_each, n_heads);
     const T* from = x + t * ldx;
     T* to = out + t * ldo;
@@ -126,36 +126,35 @@ int launch_rotary(const T* x, long long ldx, const int* positions, const unsigne
         constexpr bool HALVES = decltype(halves_tag)::value;
         // (in place the columns behind are there already)
         const int places = HALVES ? pairs / V + (in_place ? 0 : (head_dim - 2 * pairs) / V) : in_place ? (2 * pairs + V - 1) / V : head_dim / V;
-        if (places == 0) return;
+        if (places == 0) return 0;
         const long long items = static_cast<long long>(tokens) * places, blocks = (items + ROT_THREADS - 1) / ROT_THREADS;
+        if (blocks * ROT_THREADS > UINT32_MAX) return -1;             // (what one launch can have)
         const int slices = static_cast<int>(std::min<long long>(n_heads, std::max<long long>(1, 1024 / blocks)));
         const int each = (n_heads + slices - 1) / slices;
         rotary_kernel<T, V, HALVES><<<dim3(static_cast<unsigned>(blocks), (n_heads + each - 1) / each), ROT_THREADS, 0, stream>>>(
             x, out, positions, turns, tokens, pairs, n_heads, head_dim, ldx, ldo, places, each, amplitude);
+        return 0;
     };
     using std::integral_constant;
     if (interleaved) {
-        if (wide) launch(integral_constant<int, W>{}, std::false_type{});
-        else launch(integral_constant<int, 2>{}, std::false_type{});
-    } else {
-        if (wide) launch(integral_constant<int, W>{}, std::true_type{});
-        else launch(integral_constant<int, 1>{}, std::true_type{});
+        return wide ? launch(integral_constant<int, W>{}, std::false_type{}) : launch(integral_constant<int, 2>{}, std::false_type{});
     }
-    return 0;
+    return wide ? launch(integral_constant<int, W>{}, std::true_type{}) : launch(integral_constant<int, 1>{}, std::true_type{});
 }
 
 }  // namespace
 
 // out[t, h * head_dim ..] = x[t, h * head_dim ..] turned by positions[t]; out may be x. Returns 0, a HIP error code, or -1 for sizes
-// it refuses: head_dim even, 1 <= 2 * pairs <= head_dim, tokens * head_dim below 2^38.
+// it refuses: head_dim even, 1 <= 2 * pairs <= head_dim, tokens * head_dim below 2^38 and 2^32 places in all.
 extern "C" int mllm_rotary(const void* x, long long ldx, const int* positions, const unsigned long long* turns, int tokens, int pairs, int n_heads,
                            int head_dim, int interleaved, float amplitude, void* out, long long ldo, int dtype, hipStream_t stream) {
     if (tokens <= 0) return 0;
     if (n_heads < 1 || pairs < 1 || 2 * pairs > head_dim || head_dim % 2 != 0 || static_cast<long long>(tokens) * head_dim > 1ll << 38) return -1;
-    if (dtype == MLLM_F32)
-        launch_rotary(static_cast<const float*>(x), ldx, positions, turns, tokens, pairs, n_heads, head_dim, interleaved, amplitude, static_cast<float*>(out), ldo, stream);
-    else
-        launch_rotary(static_cast<const bf16_t*>(x), ldx, positions, turns, tokens, pairs, n_heads, head_dim, interleaved, amplitude, static_cast<bf16_t*>(out), ldo, stream);
+    const int rc = dtype == MLLM_F32 ? launch_rotary(static_cast<const float*>(x), ldx, positions, turns, tokens, pairs, n_heads, head_dim, interleaved, amplitude,
+                                                     static_cast<float*>(out), ldo, stream)
+                                     : launch_rotary(static_cast<const bf16_t*>(x), ldx, positions, turns, tokens, pairs, n_heads, head_dim, interleaved, amplitude,
+                                                     static_cast<bf16_t*>(out), ldo, stream);
+    if (rc != 0) return rc;
     MLLM_LAUNCH_CHECK();
     return 0;
 }

@@ -800,7 +800,7 @@ template <typename T, int NT, int RT, int K16, int NW, int KG>
 int launch(const TreeAttentionParams& p, hipStream_t stream) {
     using St = Stage<T, NT, K16, NW, KG>;
     const long long blocks = (static_cast<long long>(p.units) + 7) / 8 * 8 * p.row_tiles;
-    if (blocks > INT32_MAX) return -1;
+    if (blocks * NW * 64 > UINT32_MAX) return -1;          // (what one launch can have)
     constexpr int STATES = KG == 1 ? 0 : NW * 16 * RT * ((32 * NT + 4) * 4 + 8), LDS = std::max(St::NUMBER * St::BYTES, STATES);
     static_assert(LDS + TABLE_ENTRIES * 4 + 1024 <= 163840, "LDS of a compute unit");
     auto kernel = tree_attention_kernel<T, NT, RT, K16, NW, KG>;
@@ -852,7 +852,7 @@ int mllm_tree_attention(const void* q, long long ldq, const void* k, long long l
     if (static_cast<long long>(n_pages) * page_size > INT32_MAX || max_new < 1 || max_new > 64 * words) return -1;
     const Plan plan = plan_of(n_seqs, n_heads, n_kv_heads, head_dim, max_new, max_cached, window, dtype);
     const long long units = static_cast<long long>(n_seqs) * n_kv_heads * plan.nsplit;
-    if (units > INT32_MAX / 8 || (plan.nsplit > 1 && (ws == nullptr || n_seqs > 65535))) return -1;
+    if (units > INT32_MAX / 8 || (plan.nsplit > 1 && ws == nullptr)) return -1;
     const int esz = dtype == MLLM_F32 ? 4 : 2;
     int bits = 0;
     while ((1ll << bits) < page_size) ++bits;
@@ -874,7 +874,7 @@ int mllm_tree_attention(const void* q, long long ldq, const void* k, long long l
     const int rc = dtype == MLLM_F32 ? dispatch<float>(p, plan, stream) : dispatch<bf16_t>(p, plan, stream);
     if (rc != 0) return rc;
     if (plan.nsplit > 1) {
-        const dim3 grid(max_new, n_seqs, std::min(64, (n_heads * (head_dim / 4) + 255) / 256));
+        const dim3 grid(max_new, n_seqs, std::min(64, (n_heads * (head_dim / 4) + 255) / 256));          // (split: 1,024 workgroups at most, so as many sequences)
         if (dtype == MLLM_F32) tree_attention_join_kernel<float><<<grid, 256, 0, stream>>>(p);
         else tree_attention_join_kernel<bf16_t><<<grid, 256, 0, stream>>>(p);
     }
