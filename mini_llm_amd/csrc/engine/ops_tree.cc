@@ -25,6 +25,30 @@ static void need_pool(int64_t n_pages, int64_t page_size, const char* what) {
     if (n_pages < 1 || page_size < 1 || n_pages > INT_MAX / page_size) fail("%s: %lld pages of %lld rows", what, (long long)n_pages, (long long)page_size);
 }
 
+// (every sequence looks at the others', so that the work grows with the square of their number)
+static constexpr int MOST_SEQS = 65536;
+static void need_seqs(int n_seqs, const char* what) {
+    if (n_seqs > MOST_SEQS) fail("%s: %d sequences (at most %d)", what, n_seqs, MOST_SEQS);
+}
+
+// Arrays of one call. What one workgroup writes another may read, or write too: outputs lie apart from inputs and from each other.
+struct Span {
+    const char* name;
+    const void* at;
+    int64_t bytes;
+};
+template <size_t N, size_t M>
+static void need_apart(const char* what, const Span (&outs)[N], const Span (&ins)[M]) {
+    auto check_two = [&](const Span& a, const Span& b) {
+        const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+        if (a.at != nullptr && b.at != nullptr && a.bytes > 0 && b.bytes > 0 && x < y + b.bytes && y < x + a.bytes) fail("%s: %s shares memory with %s", what, a.name, b.name);
+    };
+    for (size_t i = 0; i < N; ++i) {
+        for (size_t j = i + 1; j < N; ++j) check_two(outs[i], outs[j]);
+        for (const Span& in : ins) check_two(outs[i], in);
+    }
+}
+
 int tree_max_nodes() { return mllm_tree_max_nodes(); }
 
 void step_maps(const StepMapsArgs& a, hipStream_t stream) {
@@ -42,6 +66,12 @@ void step_maps(const StepMapsArgs& a, hipStream_t stream) {
         if (a.ancestors == nullptr || a.words < (a.max_new + 63) / 64 || a.words > tree_max_nodes() / 64)
             fail("step_maps: trees of up to %d nodes need %d words of ancestors a node, not %d", a.max_new, (a.max_new + 63) / 64, a.words);
     }
+    need_seqs(a.n_seqs, "step_maps");
+    const int64_t n = 4ll * a.n_seqs, t = 4ll * a.tokens;
+    need_apart("step_maps", {{"cu_q", a.cu_q, n + 4}, {"cached", a.cached, n}, {"ctx_len", a.ctx_len, n}, {"token_seq", a.token_seq, t}, {"positions", a.positions, t},
+                             {"slots", a.slots, t}, {"block_tables", a.block_tables, n * a.max_blocks}, {"ancestors", a.ancestors, a.parents == nullptr ? 0 : 2 * t * a.words}},
+               {{"rows", a.rows, n}, {"n_new", a.n_new, n}, {"lengths", a.lengths, 4ll * a.n_requests},
+                {"pages", a.pages, 4 * ((a.n_requests - 1) * a.ld_pages + a.max_blocks)}, {"parents", a.parents, t}});
     check(mllm_step_maps(a.rows, a.n_new, a.lengths, a.pages, a.ld_pages, a.parents, a.n_seqs, a.n_requests, a.tokens, a.page_size, a.n_pages, a.max_blocks,
                          a.max_new, a.words, a.cu_q, a.cached, a.ctx_len, a.token_seq, a.positions, a.slots, a.block_tables, a.ancestors, stream), "step_maps");
 }
@@ -85,6 +115,7 @@ static void check_tree_attention(const TreeAttentionArgs& a) {
         fail("tree_attention: block tables, cached lengths, sequence bounds and ancestors are needed");
     if (a.words < 1 || a.words > tree_max_nodes() / 64 || a.max_new < 1 || a.max_new > 64 * a.words)
         fail("tree_attention: %d words of ancestors for trees of up to %d nodes (at most %d)", a.words, a.max_new, tree_max_nodes());
+    need_seqs(a.n_seqs, "tree_attention");
     if (a.max_cached < 0 || a.window < 0) fail("tree_attention: max_cached=%d, window=%d", a.max_cached, a.window);
     if (a.window > 0 && a.positions == nullptr) fail("tree_attention: positions are needed with a window");
     for (const Tensor2* t : {&a.q, &a.k, &a.v, &a.k_pages, &a.v_pages})
@@ -117,6 +148,11 @@ void tree_accept(const TreeAcceptArgs& a, hipStream_t stream) {
         a.kept == nullptr || a.path == nullptr || a.next == nullptr || a.slots == nullptr)
         fail("tree_accept: an array is missing");
     if (a.lengths != nullptr && a.rows == nullptr && a.n_seqs > a.n_requests) fail("tree_accept: %d sequences without rows, %d lengths", a.n_seqs, a.n_requests);
+    need_seqs(a.n_seqs, "tree_accept");
+    const int64_t n = 4ll * a.n_seqs, t = 4ll * a.tokens;
+    need_apart("tree_accept", {{"kept", a.kept, n}, {"path", a.path, n * a.max_new}, {"next_token", a.next, n}, {"slots", a.slots, t}, {"lengths", a.lengths, 4ll * a.n_requests}},
+               {{"choices", a.choices, t}, {"ids", a.ids, t}, {"parents", a.parents, t}, {"cu_q", a.cu_q, n + 4}, {"cached", a.cached, n},
+                {"block_tables", a.block_tables, n * a.max_blocks}, {"rows", a.rows, n}});
     check(mllm_tree_accept(a.choices, a.ids, a.parents, a.cu_q, a.cached, a.block_tables, a.rows, a.n_seqs, a.tokens, a.page_size, a.n_pages, a.max_blocks,
                            a.max_new, a.n_requests, a.kept, a.path, a.next, a.slots, a.lengths, stream), "tree_accept");
 }

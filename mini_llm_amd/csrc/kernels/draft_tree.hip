@@ -177,12 +177,17 @@ __global__ void __launch_bounds__(TREE_THREADS) tree_accept_kernel(TreeAcceptPar
         if (place >= 0) path[place] = first + tid;
         if (place == kept - 1) a.next[b] = choice_s[tid];
     }
+    // (of several sequences of one request the last one's length stands)
+    int later = 0;
+    if (a.lengths != nullptr && a.rows != nullptr)
+        for (int i = b + 1 + tid; i < a.n_seqs; i += threads) later |= a.rows[i] == a.rows[b];
+    later = __syncthreads_or(later);
     for (int i = kept + tid; i < a.max_new; i += threads) path[i] = -1;
     for (int i = n + tid; i < all; i += threads) a.slots[first + i] = -1;
     if (tid == 0) {
         a.kept[b] = kept;
         if (kept == 0) a.next[b] = -1;
-        if (a.lengths != nullptr) {
+        if (a.lengths != nullptr && !later) {
             const int r = a.rows != nullptr ? a.rows[b] : b;
             if (static_cast<unsigned>(r) < static_cast<unsigned>(a.n_requests)) a.lengths[r] = cached + kept;
         }

@@ -732,8 +732,14 @@ class StepMaps:
         self.token_seq, self.positions, self.slots = zeros(tokens), zeros(tokens), zeros(tokens)
         self.block_tables = zeros(n_seqs, max_blocks)
         self.ancestors = torch.zeros((tokens, self.words), dtype=torch.int64, device=device) if tree else None
+        # (the kernel writes to these addresses: the arrays stay the object's own as long as it lives)
         self.addresses = tuple(0 if t is None else t.data_ptr() for t in (self.cu_q, self.cached, self.ctx_len, self.token_seq, self.positions, self.slots,
                                                                           self.block_tables, self.ancestors))
+
+    def __setattr__(self, name, value):
+        if "addresses" in self.__dict__:
+            raise AttributeError(f"step maps keep their arrays: copy into '{name}'")
+        object.__setattr__(self, name, value)
 
 
 def step_maps(maps: StepMaps, rows: Optional[torch.Tensor], n_new: torch.Tensor, lengths: torch.Tensor, pages: torch.Tensor, page_size: int,
@@ -745,7 +751,7 @@ def step_maps(maps: StepMaps, rows: Optional[torch.Tensor], n_new: torch.Tensor,
     Without ``parents`` the tokens follow one another: positions from lengths[r] on, slots their page rows. With ``parents`` (int32
     [tokens], needs maps made with ``tree=True``) they are a tree each: positions are lengths[r] + depth, slots -1 (``tree_accept``
     says later where the kept ones go), ancestors the sets that ``tree_attention`` takes; a parent that does not stand in front of its
-    child counts as none. More than ``max_new`` tokens of a sequence, or more than ``tokens`` together, are left out (cu_q says how
+    child counts as none. The maps' arrays lie apart from the inputs. More than ``max_new`` tokens of a sequence, or more than ``tokens`` together, are left out (cu_q says how
     many are in). A position beyond ``max_blocks``, or whose page is none of the ``n_pages``, has slot -1. Tokens behind the last sequence get
     sequence 0, position 0, slot -1 and no ancestors."""
     B, T, blocks, mine = maps.n_seqs, maps.tokens, maps.max_blocks, maps.addresses
@@ -884,7 +890,8 @@ def tree_accept(choices: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor,
     of its children whose token was chosen at it does. Writes, all int32: kept [n_seqs], the number of nodes that stand; path [n_seqs, max_new],
     their rows, -1 behind them; next_token [n_seqs], the choice at the last (a sequence without nodes: 0, -1, -1); slots [T], the page row of
     each node that stands (position cached[b] + its place on the path), -1 for the others and the rows of no sequence: what ``kv_append`` takes.
-    With ``lengths`` (int32 [requests]): lengths[rows[b]] = cached[b] + kept[b] (``rows`` None: b). A page that is none of the ``n_pages`` gives slot -1."""
+    With ``lengths`` (int32 [requests]): lengths[rows[b]] = cached[b] + kept[b] (``rows`` None: b; of sequences of one request the last counts). Outputs lie
+    apart from the inputs and each other. A page that is none of the ``n_pages`` gives slot -1."""
     T, B = choices.numel(), cached.numel()
     tokens = [_counted(t, n, T) for t, n in ((choices, "choices"), (ids, "ids"), (parents, "parents"), (slots, "slots"))]
     at_cached, at_kept, at_next, at_cu = _counted(cached, "cached", B), _counted(kept, "kept", B), _counted(next_token, "next_token", B), _counted(cu_q, "cu_q", B + 1)

@@ -208,3 +208,51 @@ def test_plain_attention():
     out = plain_tree.attention(q, torch.tensor([[0.0], [5.0]]), torch.tensor([[8.0], [2.0]]), 1, 1, 1, torch.tensor([[0.0], [math.nan]]), torch.tensor([[4.0], [math.nan]]), 1, [[0, 1]], [1],
                                [0, 2], [[1], [0]], [1, 2], 1.0, 0)[0]
     assert out.tolist() == [[6.0], [4.0]]
+
+
+# -- arrays that share memory, and more sequences than a call takes ------------------------------------------------------------------
+def native_ints(kind, op, sizes, **change):
+    """A native call whose arrays lie a mebibyte apart, but for those of `change`."""
+    a = kind(**dict({n: (i + 1) << 20 for i, n in enumerate(n for n, t in kind._fields_ if t is ctypes.c_void_p)}, **sizes) | change)
+    ops._ok(getattr(ops.engine_library(), op)(ctypes.byref(a), None))
+
+
+MAPS_SIZES = dict(ld_pages=3, n_seqs=2, n_requests=5, tokens=8, page_size=16, n_pages=9, max_blocks=3, max_new=4, words=1)
+ACCEPT_SIZES = dict(n_seqs=2, tokens=6, page_size=16, n_pages=9, max_blocks=4, max_new=3, n_requests=2)
+
+
+def test_step_maps_into_its_inputs_is_refused():
+    """Several workgroups read a request's length: the context lengths of the step before cannot be this step's lengths in place."""
+    names = [n for n, t in ops.StepMapsC._fields_ if t is ctypes.c_void_p]
+    for out in ("cu_q", "cached", "ctx_len", "token_seq", "positions", "slots", "block_tables", "ancestors"):
+        for other in names:
+            if other != out:
+                with pytest.raises(ops.KernelError, match="shares memory"):
+                    native_ints(ops.StepMapsC, "mllm_op_step_maps", MAPS_SIZES, **{out: (names.index(other) + 1) << 20})
+    with pytest.raises(ops.KernelError, match="ctx_len shares memory with lengths"):
+        native_ints(ops.StepMapsC, "mllm_op_step_maps", MAPS_SIZES, ctx_len=(3 << 20) + 4 * 4)
+
+
+def test_tree_accept_into_its_inputs_is_refused():
+    names = [n for n, t in ops.TreeAcceptC._fields_ if t is ctypes.c_void_p]
+    for out in ("kept", "path", "next", "slots", "lengths"):
+        for other in names:
+            if other != out:
+                with pytest.raises(ops.KernelError, match="shares memory"):
+                    native_ints(ops.TreeAcceptC, "mllm_op_tree_accept", ACCEPT_SIZES, **{out: (names.index(other) + 1) << 20})
+
+
+def test_more_sequences_than_a_call_takes_are_refused():
+    with pytest.raises(ops.KernelError, match="65537 sequences"):
+        native_ints(ops.StepMapsC, "mllm_op_step_maps", MAPS_SIZES, n_seqs=65537)
+    with pytest.raises(ops.KernelError, match="65537 sequences"):
+        native_ints(ops.TreeAcceptC, "mllm_op_tree_accept", ACCEPT_SIZES, n_seqs=65537)
+    with pytest.raises(ops.KernelError, match="65537 sequences"):
+        native_attention(n_seqs=65537)
+
+
+def test_step_maps_keep_their_arrays():
+    """The kernel writes to addresses taken once: an array put in another's place would not be written, and the one gone would be."""
+    m = ops.StepMaps(2, 8, 3, 4, tree=True, device="cpu")
+    with pytest.raises(AttributeError, match="keep their arrays"):
+        m.slots = i32(8)

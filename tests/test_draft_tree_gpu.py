@@ -516,6 +516,19 @@ class Model:
         return chosen, rows, logits
 
 
+def test_tree_accept_of_one_request_twice(ops):
+    """Of several sequences of one request the last one's length stands, whatever the order of arrival: 300 sequences of 7 requests."""
+    B, R = 300, 7
+    rows = [(5 * b + b // 11) % (R + 1) for b in range(B)]                     # (row R names nobody)
+    cached = [10 * b for b in range(B)]
+    kept, path, following, slots, lengths = (torch.full(s, -7, dtype=torch.int32, device="cuda") for s in ((B,), (B, 2), (B,), (B,), (R,)))
+    for _ in range(3):
+        lengths.fill_(-7)
+        ops.tree_accept(ints([4] * B), ints([1] * B), ints([-1] * B), ints(range(B + 1)), ints(cached), ints([[3] * 200] * B), 16, 9, kept, path, following, slots, lengths, ints(rows))
+        assert lengths.tolist() == [max(cached[b] for b in range(B) if rows[b] == r) + 1 for r in range(R)]
+        assert kept.tolist() == [1] * B
+
+
 def token_by_token(ops, dtype, prompts, steps):
     m = Model(ops, dtype)
     texts, margins = [], []
