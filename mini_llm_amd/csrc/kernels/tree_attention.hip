@@ -385,7 +385,9 @@ __device__ __forceinline__ float2* split_state(const TreeAttentionParams& a, siz
     return reinterpret_cast<float2*>(a.ws + static_cast<size_t>(a.tokens) * a.n_heads * a.nsplit * a.head_dim) + pair;
 }
 
-// 16-byte piece p of row k of a stage lies at piece p ^ (k % 16), so that 16 lanes that read one piece of 16 rows meet no bank twice.
+// 16-byte piece p of row k of a stage lies at piece p ^ (k % 16, its bit 3 turned by its bit 2). A 16-byte read serves lanes 0-3, 12-15 and 20-27 at
+// once, then the others of 32 alike: of keys that is one piece of rows 0-3 and 12-15 and its neighbour of rows 4-11, of values eight pieces of a row and
+// the other eight of the row four further on: no bank is met twice. (By k % 16 alone the values' reads took twice as long, a third of all LDS cycles.)
 constexpr int TABLE_ENTRIES = 2048;
 template <typename T, int NT, int K16, int NW, int KG>
 struct Stage {
@@ -412,6 +414,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     using St = Stage<T, NT, K16, NW, KG>;
     constexpr int KT = S::KT, KEYS = S::KEYS, CH = S::CH, TILES = S::TILES, PIECES = St::PIECES, SK = St::KEYS, RG = NW / KG, PITCH = 32 * NT + 4;
     constexpr int TURN = std::min(PIECES, 16) - 1;
+    auto turned = [](int k) { return (k ^ (k & 4) << 1) & TURN; };
     // the stages [keys, values][SK][PIECES * 16]; at the end the states [wavefront][16 RT][PITCH], then their maxima and sums
     extern __shared__ __attribute__((aligned(16))) unsigned char stage_s[];
     __shared__ int table_s[TABLE_ENTRIES];
@@ -476,7 +479,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     unsigned offset[St::LOADS];
 #pragma unroll
     for (int i = 0; i < St::LOADS; ++i) {
-        const int k = wave * St::MINE + i * St::PER_LOAD + lane / PIECES, piece = (lane % PIECES) ^ (k & TURN);
+        const int k = wave * St::MINE + i * St::PER_LOAD + lane / PIECES, piece = (lane % PIECES) ^ turned(k);
         offset[i] = (lane / PIECES) * a.page_pitch + (16 * piece < row_bytes ? 16 * piece : 0);
     }
     const unsigned char *k_head = reinterpret_cast<const unsigned char*>(a.k_pages) + head, *v_head = reinterpret_cast<const unsigned char*>(a.v_pages) + head;
@@ -528,14 +531,14 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
         const size_t k_pitch = of_nodes ? a.ldk : a.page_pitch, v_pitch = of_nodes ? a.ldv : a.page_pitch;
 #pragma unroll 1
         for (int i = 0; i < St::LOADS; ++i) {
-            const int k = i * St::PER_LOAD + lane / PIECES, piece = lane % PIECES ^ ((wave * St::MINE + k) & TURN);
+            const int k = i * St::PER_LOAD + lane / PIECES, piece = (lane % PIECES) ^ turned(wave * St::MINE + k);
             const int off = 16 * piece < row_bytes ? 16 * piece : 0;
             const size_t from = __shfl(row, k, 64);
             load_to_lds(kb, from * k_pitch + off, to + 1024 * i);
             load_to_lds(vb, from * v_pitch + off, to + St::MATRIX + 1024 * i);
         }
     };
-    auto place_of = [&](int k, int piece) { return 16 * (piece ^ (k & TURN)); };
+    auto place_of = [&](int k, int piece) { return 16 * (piece ^ turned(k)); };
 
     // One loop over the wavefront's tiles of all stages: in two loops, one in the other, the outputs would be copied from the one's registers
     // to the other's for every tile. (A wavefront whose rows lie behind the last works on the last again, and writes nothing.)
