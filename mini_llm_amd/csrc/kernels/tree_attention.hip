@@ -17,9 +17,9 @@
 //   S^T = K Q^T   the lane with row c, group G (lane = 16 G + c) takes key c of each 16, 16 bytes at 64 i + 16 G of its row: the product's k
 //                 index runs over the columns in an order of its own, the same for queries and keys;
 //   O^T = V^T P^T the lane has the weights of keys 4 G .. 4 G + 3 of each 16 from the first product, in the place where the second wants
-//                 them. As the other operand it takes, of just these keys, 16 (8, 4) bytes at the same place c of a block of 256 (128, 64) bytes:
-//                 column m of the product's tile x is column E m + x of the block, E elements to 16 bytes. In 32 bits the words are
-//                 the operand; in bfloat16 a byte permutation joins two keys' halves, one instruction a register, shared by all rows.
+//                 them, and takes the values of just these keys in 16 columns as the other operand. In bfloat16 these come out of LDS turned by
+//                 the read itself; in 32 bits a lane reads 16 (8) bytes at the same place c of a block of 256 (128) bytes: column m of the
+//                 product's tile x is column E m + x of the block, E words to a read.
 // Softmax statistics, sums and outputs are fp32; the weights are rounded to the values' type for the second product (in bfloat16: by half a step,
 // which averages over the keys; the sum is over the weights before they are rounded).
 #include "common.h"
@@ -33,6 +33,10 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <typename V> __device__ __forceinline__ V from_lds(unsigned at) { return *(const __attribute__((address_space(3))) V*)(at); }
 
 struct TreeAttentionParams {
     const char *q, *k, *v, *k_pages, *v_pages;
@@ -56,12 +60,13 @@ template <typename T, int NT, int KEY_GROUPS_OF_16>
 struct Shape {
     static constexpr int KT = KEY_GROUPS_OF_16;            // 16-key groups of a tile (bfloat16: a product step of values takes two)
     static constexpr int KEYS = 16 * KT;
-    static constexpr int CH = NT * sizeof(T) / 2;          // 64-byte pieces of a row; words of a value row in a lane
+    static constexpr int CH = NT * sizeof(T) / 2;          // 64-byte pieces of a row
     static constexpr int PER = 4 / sizeof(T);              // elements of a word
     static constexpr int TILES = 2 * NT;                   // 16-column tiles of the output
     static constexpr int LEAST = NT / 2;                   // heads are wider than 32 LEAST
     static_assert((NT & (NT - 1)) == 0, "a power of two");
-    static constexpr int BLOCK = std::min(CH, 4);          // words of a lane that lie together
+    static constexpr int BLOCK = std::min(CH, 4);          // 32 bits: words of a value row that lie together in a lane
+    static constexpr int WORDS = 4 * KT / PER;             // words of a lane's keys in a column
 };
 
 // Ones (1 in the lowest bit of each element) where a word's elements are not finite. In whole-number arithmetic on all elements of the word at
@@ -154,7 +159,7 @@ struct Rows {
             }
     }
 
-    // The second product: into(x, rt, product) for every tile x of columns and 16 rows, of the words word(j, w) of the lane's keys j and the weights
+    // The second product: into(x, rt, product) for every tile x of columns and 16 rows, of the words word(j, x) of the lane's keys (PER in a word) and the weights
     // weight(rt, j).
     // In bfloat16 added(rt, product) is handed the product of ones with the weights, whose rows are the weights' sum.
     template <bool ONE_BY_ONE, typename V, typename W, typename F, typename A>
@@ -174,27 +179,19 @@ struct Rows {
                         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones), __builtin_bit_cast(bf16x8, pb[rt]), c, 0, 0, 0);
                     });
 #pragma unroll
-                for (int w = 0; w < CH; ++w) {
-                    uint32_t vw[8];
+                for (int x = 0; x < TILES; ++x) {
+                    const uint4 va = make_uint4(word(h / 2, x), word(h / 2 + 1, x), word(h / 2 + 2, x), word(h / 2 + 3, x));
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) vw[j] = word(h + j, w);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t sel = e == 0 ? 0x05040100u : 0x07060302u;
-                        const uint4 va = make_uint4(__builtin_amdgcn_perm(vw[1], vw[0], sel), __builtin_amdgcn_perm(vw[3], vw[2], sel),
-                                                    __builtin_amdgcn_perm(vw[5], vw[4], sel), __builtin_amdgcn_perm(vw[7], vw[6], sel));
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-                            into(2 * w + e, rt, [&](f32x4 c) {
-                                return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, pb[rt]), c, 0, 0, 0);
-                            });
-                    }
+                    for (int rt = 0; rt < RT; ++rt)
+                        into(x, rt, [&](f32x4 c) {
+                            return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, pb[rt]), c, 0, 0, 0);
+                        });
                     if (ONE_BY_ONE) __builtin_amdgcn_sched_barrier(0);
                 }
             }
         } else {
 #pragma unroll
-            for (int w = 0; w < CH; ++w) {
+            for (int w = 0; w < TILES; ++w) {
                 float vw[4 * KT];
 #pragma unroll
                 for (int j = 0; j < 4 * KT; ++j) vw[j] = __builtin_bit_cast(float, word(j, w));
@@ -275,18 +272,18 @@ struct Rows {
     __device__ __forceinline__ float sum_of(int rt) const { return sizeof(T) == 4 ? rows_sum(sum[rt][0]) : sum[rt][0]; }
 
     // A tile whose keys all rows see, from its products on, with the lane's words of its values.
-    __device__ __forceinline__ void take(float (&p)[RT][4 * KT], float scale, const uint32_t (&v)[4 * KT][CH]) {
+    __device__ __forceinline__ void take(float (&p)[RT][4 * KT], float scale, const uint32_t (&v)[TILES][S::WORDS]) {
         // (The weights' chain of dependent instructions goes first on the unit, so that the other wavefront's products run beside it: 256 rows of 128
         // columns over 8,192 positions, 32 sequences: 310 > 288 us; the products first: 290; products and scores first: 300.)
         __builtin_amdgcn_s_setprio(1);
         weights(p, scale);
         __builtin_amdgcn_s_setprio(0);
-        weigh<false>([&](int j, int w) { return v[j][w]; }, [&](int rt, int j) { return p[rt][j]; },
+        weigh<false>([&](int j, int w) { return v[w][j]; }, [&](int rt, int j) { return p[rt][j]; },
                      [&](int x, int rt, auto&& product) { o[x][rt] = product(o[x][rt]); }, [&](int rt, auto&& product) { sum[rt] = product(sum[rt]); });
     }
     // Any tile: keys [at0, at0 + KEYS) of the cache, or of the nodes; `valid` has a bit for each that exists. stored(j, w) gives a word of the values again.
     template <typename W>
-    __device__ __forceinline__ void take_some(float (&p)[RT][4 * KT], const uint32_t (&v)[4 * KT][CH], const TreeAttentionParams& a, bool of_nodes, int at0,
+    __device__ __forceinline__ void take_some(float (&p)[RT][4 * KT], const uint32_t (&v)[TILES][S::WORDS], const TreeAttentionParams& a, bool of_nodes, int at0,
                                               unsigned long long valid, int first, int nodes, W&& stored) {
         const int G = threadIdx.x % 64 / 16;
         unsigned mine = 0;                   // which of the lane's keys exist
@@ -318,22 +315,24 @@ struct Rows {
         // A key that does not exist has some other row's values. A value that is not finite, in a tile of which some rows see less than others,
         // would reach those that do not see it as zero times it: the finite values are weighed as ever, and whether a row gives weight to a NaN,
         // +inf or -inf of a column is a product of ones and zeros. (For these products the words are read anew, which keeps them out of the registers.)
-        auto exists = [&](int j) { return 0u - (mine >> j & 1); };
+        auto exists = [&](int j) {           // (of the keys of word j)
+            return sizeof(T) == 2 ? (mine >> 2 * j & 1 ? 0xffffu : 0u) | (mine >> 2 * j & 2 ? 0xffff0000u : 0u) : 0u - (mine >> j & 1);
+        };
         auto weight = [&](int rt, int j) { return p[rt][j]; };
         auto add = [&](int x, int rt, auto&& product) { o[x][rt] = product(o[x][rt]); };
         uint32_t odd = 0;
 #pragma unroll
-        for (int j = 0; j < 4 * KT; ++j) {
+        for (int j = 0; j < S::WORDS; ++j) {
             uint32_t each = 0;
 #pragma unroll
-            for (int w = 0; w < CH; ++w) each |= not_finite(v[j][w], T{});
+            for (int w = 0; w < TILES; ++w) each |= not_finite(v[w][j], T{});
             odd |= each & exists(j);
         }
         auto added = [&](int rt, auto&& product) { sum[rt] = product(sum[rt]); };
         int plain = !__any(odd != 0);
         asm volatile("" : "+v"(plain));          // (a lane's register, as where this function is called)
         if (plain) {
-            weigh<true>([&](int j, int w) { return v[j][w] & exists(j); }, weight, add, added);
+            weigh<true>([&](int j, int w) { return v[w][j] & exists(j); }, weight, add, added);
             return;
         }
         auto word = [&](int j, int w) { return stored(j, w) & exists(j); };
@@ -351,8 +350,8 @@ struct Rows {
         }
     }
 
-    // o[x][rt][i] stands in column column(x) + EACH (4 G + i) of its row: EACH elements a lane has in a block.
-    static constexpr int EACH = S::BLOCK * S::PER;
+    // o[x][rt][i] stands in column column(x) + EACH (4 G + i) of its row.
+    static constexpr int EACH = sizeof(T) == 2 ? 1 : S::BLOCK;
     __device__ __forceinline__ static constexpr int column(int x) { return x / EACH * 16 * EACH + x % EACH; }
 };
 
@@ -385,9 +384,10 @@ __device__ __forceinline__ float2* split_state(const TreeAttentionParams& a, siz
     return reinterpret_cast<float2*>(a.ws + static_cast<size_t>(a.tokens) * a.n_heads * a.nsplit * a.head_dim) + pair;
 }
 
-// 16-byte piece p of row k of a stage lies at piece p ^ (k % 16, its bit 3 turned by its bit 2). A 16-byte read serves lanes 0-3, 12-15 and 20-27 at
-// once, then the others of 32 alike: of keys that is one piece of rows 0-3 and 12-15 and its neighbour of rows 4-11, of values eight pieces of a row and
-// the other eight of the row four further on: no bank is met twice. (By k % 16 alone the values' reads took twice as long, a third of all LDS cycles.)
+// 16-byte piece p of row k of a stage lies at piece p ^ turned(k). A 16-byte read serves lanes 0-3, 12-15 and 20-27 at once, then the others of 32 alike:
+// of keys that is one piece of rows 0-3 and 12-15 and its neighbour of rows 4-11; the values' turning read serves 32 lanes, 32 bytes of each of eight
+// rows; a 16-byte read of values has eight pieces of a row and the other eight of the row four further on. None meets a bank twice. (By k % 16 alone the
+// reads of values took twice as long, a third of all LDS cycles.)
 constexpr int TABLE_ENTRIES = 2048;
 template <typename T, int NT, int K16, int NW, int KG>
 struct Stage {
@@ -413,10 +413,12 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     using S = Shape<T, NT, K16>;
     using St = Stage<T, NT, K16, NW, KG>;
     constexpr int KT = S::KT, KEYS = S::KEYS, CH = S::CH, TILES = S::TILES, PIECES = St::PIECES, SK = St::KEYS, RG = NW / KG, PITCH = 32 * NT + 4;
-    constexpr int TURN = std::min(PIECES, 16) - 1;
-    auto turned = [](int k) { return (k ^ (k & 4) << 1) & TURN; };
+    auto turned = [](int k) {
+        if (PIECES < 16) return k & (PIECES - 1);
+        return sizeof(T) == 2 ? (k & 7) << 1 ^ (k & 8 ? 9 : 0) : (k ^ (k & 4) << 1) & 15;
+    };
     // the stages [keys, values][SK][PIECES * 16]; at the end the states [wavefront][16 RT][PITCH], then their maxima and sums
-    extern __shared__ __attribute__((aligned(16))) unsigned char stage_s[];
+    extern __shared__ __attribute__((aligned(512))) unsigned char stage_s[];
     __shared__ int table_s[TABLE_ENTRIES];
     __shared__ unsigned long long valid_s[St::NUMBER][NW];                // of each wavefront's rows of a stage: a bit a key that exists
     Work w;
@@ -545,22 +547,36 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     constexpr int TURNS = SK / KEYS / KG;
     // Everything comes from LDS a phase before it is multiplied: a tile's keys while the tile in front of it is weighed (its stage has come by then),
     // its values while its own products are made.
-    int key_at[CH], value_at[4][CH];        // of the lane's pieces of 16 rows; those of the next 16 lie 16 rows behind
+    constexpr bool SHORT = sizeof(T) == 2;
+    // Where the lane's pieces of 16 rows lie; those of the next 16 lie 16 rows behind. A row starts at a multiple of its (two) powers of two of bytes, so a
+    // piece further on in it is the first one's address with some bits turned.
+    static_assert(St::BYTES % 512 == 0 && KEYS * St::ROW % 512 == 0 && St::ROW <= (SHORT ? 512 : 1024), "rows start at multiples of their size");
+    const int key_at = c16 * St::ROW + place_of(c16, G);
+    int value_at[SHORT ? 1 : 4 * CH];
+    if constexpr (SHORT) {
+        value_at[0] = St::MATRIX + (4 * G + c16 / 4) * St::ROW + place_of(4 * G + c16 / 4, c16 % 4 / 2) + c16 % 2 * 8;
+    } else {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) key_at[c] = c16 * St::ROW + place_of(c16, 4 * c + G);
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int x = 0; x < CH; ++x) {
-            const int row = 4 * G + i, byte = 64 * (x / S::BLOCK * S::BLOCK) + 4 * S::BLOCK * c16;
-            value_at[i][x] = St::MATRIX + row * St::ROW + place_of(row, byte / 16) + byte % 16;
-        }
+            for (int x = 0; x < CH; ++x) {
+                const int row = 4 * G + i, byte = 64 * (x / S::BLOCK * S::BLOCK) + 4 * S::BLOCK * c16;
+                value_at[i * CH + x] = St::MATRIX + row * St::ROW + place_of(row, byte / 16) + byte % 16;
+            }
+    }
+    // (16 bits) Of two words of column 16 x + c16 the keys 4 G .. 4 G + 3 of a 16: the sixteen lanes of a G give the addresses of four keys' 32 bytes in pieces of
+    // eight, and each gets a column of them.
+    auto two_words = [&](unsigned keys, int kt, int x) {
+        const unsigned at = ((keys + value_at[0]) ^ (32 * x)) + kt * 16 * St::ROW;
+        return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at)));
+    };
     uint4 k[KT][CH];
-    auto read_keys = [&](const unsigned char* keys) {
+    auto read_keys = [&](unsigned keys) {
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int c = 0; c < CH; ++c) k[kt][c] = *reinterpret_cast<const uint4*>(keys + key_at[c] + kt * 16 * St::ROW);
+            for (int c = 0; c < CH; ++c)
+                k[kt][c] = __builtin_bit_cast(uint4, from_lds<u32x4>((St::ROW <= 512 ? (keys + key_at) ^ (64 * c) : keys + c16 * St::ROW + place_of(c16, 4 * c + G)) + kt * 16 * St::ROW));
     };
     const int steps = (end - begin) * TURNS;
     // (not unrolled: code that runs once waits for its instructions to come)
@@ -569,34 +585,42 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
         if (begin + i < end) ask(begin + i);
     if (steps > 0) {
         wait_tiles_and_meet<St::NUMBER - 3, 2 * St::LOADS>(min(St::NUMBER - 3, end - 1 - begin));
-        read_keys(stage_s + kg * (KEYS * St::ROW));
+        read_keys(lds0 + kg * (KEYS * St::ROW));
     }
     // (tiles from seen_begin to whole_end: every row sees all keys)
     const int seen_begin = a.window > 0 ? (max(r.low_most, 0) + SK - 1) / SK - first_tile : 0;
     int turn = 0, tile = begin, place = 0;
     for (int step = 0; step < steps; ++step) {
-        const unsigned char* keys = stage_s + place * St::BYTES + (turn * KG + kg) * (KEYS * St::ROW);
+        const unsigned keys = lds0 + place * St::BYTES + (turn * KG + kg) * (KEYS * St::ROW);
         if (turn == 0) {
             // the next stage has come (those behind it may be on their way), and all have read the one in front of this
             wait_tiles_and_meet<St::NUMBER - 3, 2 * St::LOADS>(max(0, min(St::NUMBER - 3, end - 2 - tile)));
             if (tile + St::NUMBER - 1 < end) ask(tile + St::NUMBER - 1);
         }
-        uint32_t v[4 * KT][CH];
+        uint32_t v[TILES][S::WORDS];
+        if constexpr (SHORT) {
 #pragma unroll
-        for (int j = 0; j < 4 * KT; ++j)
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int x = 0; x < CH; x += S::BLOCK) {
-                const unsigned char* at = keys + value_at[j % 4][x] + j / 4 * 16 * St::ROW;
-                if (S::BLOCK == 4) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(at);
-                    v[j][x] = u.x; v[j][x + 1] = u.y; v[j][x + 2] = u.z; v[j][x + 3] = u.w;
-                } else if (S::BLOCK == 2) {
-                    const uint2 u = *reinterpret_cast<const uint2*>(at);
-                    v[j][x] = u.x; v[j][x + 1] = u.y;
-                } else {
-                    v[j][x] = *reinterpret_cast<const uint32_t*>(at);
+                for (int x = 0; x < TILES; ++x) {
+                    const u32x2 u = two_words(keys, kt, x);
+                    v[x][2 * kt] = u.x; v[x][2 * kt + 1] = u.y;
                 }
-            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4 * KT; ++j)
+#pragma unroll
+                for (int x = 0; x < CH; x += S::BLOCK) {
+                    const unsigned at = keys + value_at[j % 4 * CH + x] + j / 4 * 16 * St::ROW;
+                    if (S::BLOCK == 4) {
+                        const u32x4 u = from_lds<u32x4>(at);
+                        v[x][j] = u.x; v[x + 1][j] = u.y; v[x + 2][j] = u.z; v[x + 3][j] = u.w;
+                    } else {
+                        const u32x2 u = from_lds<u32x2>(at);
+                        v[x][j] = u.x; v[x + 1][j] = u.y;
+                    }
+                }
+        }
         __builtin_amdgcn_sched_barrier(0);
         float p[RT][4 * KT];
         r.scores(p, row_bytes, k);
@@ -607,7 +631,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             ++tile;
             place = place + 1 == St::NUMBER ? 0 : place + 1;
         }
-        if (step + 1 < steps) read_keys(stage_s + place * St::BYTES + (turn * KG + kg) * (KEYS * St::ROW));
+        if (step + 1 < steps) read_keys(lds0 + place * St::BYTES + (turn * KG + kg) * (KEYS * St::ROW));
         __builtin_amdgcn_sched_barrier(0);
         // (The condition is kept in a lane's register: as a scalar branch, which the same one in all lanes could be, the compiler gives the outputs other
         // registers on either side of a product, and moves or spills them every time.)
@@ -630,7 +654,12 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             some = static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(some >> 32)))) << 32 |
                    static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(some)));
             r.take_some(p, v, a, of_nodes, at0 + k0, some, first, nodes, [&](int j, int x) {
-                return *reinterpret_cast<const uint32_t*>(keys + value_at[j % 4][x] + j / 4 * 16 * St::ROW + 4 * (x % S::BLOCK));
+                if constexpr (SHORT) {
+                    const u32x2 u = two_words(keys, j / 2, x);
+                    return j % 2 == 0 ? u.x : u.y;
+                } else {
+                    return from_lds<uint32_t>(keys + value_at[j % 4 * CH + x] + j / 4 * 16 * St::ROW + 4 * (x % S::BLOCK));
+                }
             });
         }
     }
@@ -646,18 +675,29 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             T* to = reinterpret_cast<T*>(a.out + t * a.ldo) + h * a.head_dim;
             const size_t pair = (static_cast<size_t>(t) * a.n_heads + h) * a.nsplit + w.split;
             float* part = a.ws + pair * a.head_dim;
+            if constexpr (SHORT) {
 #pragma unroll
-            for (int x = 0; x < TILES; x += R::EACH)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int d = R::column(x) + R::EACH * (4 * G + i);
+                for (int x = 0; x < TILES; ++x) {
+                    const int d = R::column(x) + 4 * G;
                     if (d >= a.head_dim) continue;
-#pragma unroll
-                    for (int e = 0; e < R::EACH; ++e) {
-                        if (a.nsplit == 1) to[d + e] = from_float<T>(r.o[x + e][rt][i] * inv);
-                        else part[d + e] = r.o[x + e][rt][i];
-                    }
+                    const f32x4 o = r.o[x][rt];
+                    if (a.nsplit == 1) *reinterpret_cast<uint2*>(to + d) = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
+                    else *reinterpret_cast<f32x4*>(part + d) = o;
                 }
+            } else {
+#pragma unroll
+                for (int x = 0; x < TILES; x += R::EACH)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int d = R::column(x) + R::EACH * (4 * G + i);
+                        if (d >= a.head_dim) continue;
+#pragma unroll
+                        for (int e = 0; e < R::EACH; ++e) {
+                            if (a.nsplit == 1) to[d + e] = from_float<T>(r.o[x + e][rt][i] * inv);
+                            else part[d + e] = r.o[x + e][rt][i];
+                        }
+                    }
+            }
             if (a.nsplit > 1 && G == 0) *split_state(a, pair) = make_float2(r.m[rt], sum);
         }
         return;
@@ -672,9 +712,12 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
         if (G == 0) ml_s[wave * 16 * RT + 16 * rt + c16] = make_float2(r.m[rt], sum);
         float* to = state_s + (wave * 16 * RT + 16 * rt + c16) * PITCH;
 #pragma unroll
-        for (int x = 0; x < TILES; ++x)
+        for (int x = 0; x < TILES; ++x) {
+            if constexpr (SHORT) *reinterpret_cast<f32x4*>(to + R::column(x) + 4 * G) = r.o[x][rt];
+            else
 #pragma unroll
-            for (int i = 0; i < 4; ++i) to[R::column(x) + R::EACH * (4 * G + i)] = r.o[x][rt][i];
+                for (int i = 0; i < 4; ++i) to[R::column(x) + R::EACH * (4 * G + i)] = r.o[x][rt][i];
+        }
     }
     lds_barrier();
     const int quads = a.head_dim / 4, count = min(16 * RT * RG, w.rows - group0);
