@@ -22,6 +22,17 @@
 //                 product's tile x is column E m + x of the block, E words to a read.
 // Softmax statistics, sums and outputs are fp32; the weights are rounded to the values' type for the second product (in bfloat16: by half a step,
 // which averages over the keys; the sum is over the weights before they are rounded).
+//
+// What bounds it, as measured in bfloat16 (a copy of 1 GiB reaches 5.2 TB/s, a product of 8,192 cubed 1.35 PFLOP/s):
+//   64 nodes over 31,000 positions, 25 heads of 64: 45 us, 4.5 TB/s: memory, and the join of 8 splits behind it (4 us).
+//   32 trees of up to 64 nodes over 4,096 to 8,192 positions, 32 query heads that share 8 of 128: 266 us, 0.59 PFLOP/s, 3.1 TB/s: what a unit has to do
+//   for a tile, at the clock that its power leaves. Matrix instructions are 45% of its cycles, softmax and addresses 35%; without loads from memory it takes 4% less; with the
+//   longest sequences' ends shared out to units that are done it takes as long.
+//   8 sequences of one node over 1,000 positions, 12 heads of 64: 12 us, of which 8 are a launch, three loads that wait for each other (lengths, table,
+//   keys) and the merge.
+// What the steps to this gave (us; these three calls, and one of 3 trees of 37 nodes with a window of 1,000, 10 heads of 80 that share 5): a workgroup a
+// row and head, keys straight from memory: 17,689, 101,655, 501, 732; on the matrix cores with LDS stages: 51, 313, 15, 27; the way of sharing
+// a call out by measured times: 46, 302, 12, 16; values turned by the read: 45, 266, 12, 15.
 #include "common.h"
 #include "lds_loads.h"
 
@@ -274,7 +285,7 @@ struct Rows {
     // A tile whose keys all rows see, from its products on, with the lane's words of its values.
     __device__ __forceinline__ void take(float (&p)[RT][4 * KT], float scale, const uint32_t (&v)[TILES][S::WORDS]) {
         // (The weights' chain of dependent instructions goes first on the unit, so that the other wavefront's products run beside it: 256 rows of 128
-        // columns over 8,192 positions, 32 sequences: 310 > 288 us; the products first: 290; products and scores first: 300.)
+        // columns over 8,192 positions, 32 sequences: in short runs 310 > 288 us, in long ones 312 > 301; the products first: 290; products and scores first: 300.)
         __builtin_amdgcn_s_setprio(1);
         weights(p, scale);
         __builtin_amdgcn_s_setprio(0);

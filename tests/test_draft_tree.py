@@ -256,3 +256,12 @@ def test_step_maps_keep_their_arrays():
     m = ops.StepMaps(2, 8, 3, 4, tree=True, device="cpu")
     with pytest.raises(AttributeError, match="keep their arrays"):
         m.slots = i32(8)
+
+
+def test_kernels_of_drafted_trees_keep_no_register_in_scratch():
+    """Tree attention's outputs stay in one set of registers through the loop only as long as no branch in it is the scalar unit's; what spills waits for memory."""
+    from test_kernel_resources import kernels
+    for library, least in (("tree_attention", 30), ("rotary", 8), ("draft_tree", 2)):
+        found = kernels(library)
+        assert len(found) >= least
+        assert {k: n for k, n in found.items() if n} == {}
