@@ -822,8 +822,8 @@ constexpr Way NARROW[] = {{1, 4, 4}, {1, 8, 4}, {1, 8, 2}, {2, 8, 2}, {2, 8, 1}}
 
 // Of every way and number of splits the one whose time is the least by a sum of what was measured, in us: a step (a wavefront's keys of a
 // stage) takes 0.8 and its products, workgroups beyond the compute units take turns, all stages together come at 4.2 TB/s, and a
-// join takes 2.5 and 0.2 a split. The numbers were fitted to 64 calls in all ways of sharing them out; of 64 others the times taken lie 4% above the
-// best on average (75% at most) where fixed bounds on rows and keys lay 21% above it (158% at most).
+// join takes 2.5 and 0.2 a split. The numbers were fitted to 64 calls in all ways of sharing them out: the times taken lie 4% above the best on average
+// where fixed bounds on rows and keys lay 21% above it. Of 174 other calls, drawn later, they lie 3 to 5% above it (55% at most).
 Plan plan_of(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_new, int max_cached, int window, int dtype) {
     const bool f32 = dtype == MLLM_F32;
     const int nt = head_dim <= 32 ? 1 : head_dim <= 64 ? 2 : head_dim <= 128 ? 4 : 8, keys = f32 ? 16 : 32;
