@@ -245,6 +245,23 @@ def test_tree_attention_is_right_whatever_longest_cache_it_is_told(ops, dtype, h
     c.check(c.call(ops, c.device(), max_cached=hint))
 
 
+F32, BF16 = torch.float32, torch.bfloat16
+WAYS = [(F32, 8, 9, 3, 11, 16, 13500), (F32, 7, 1, 1, 17, 16, 12990), (F32, 8, 9, 5, 39, 16, 13719), (F32, 8, 1, 5, 13, 16, 14134), (F32, 8, 9, 4, 9, 64, 30013), (F32, 8, 1, 1, 17, 64, 26878),
+        (F32, 8, 5, 7, 55, 64, 15668), (F32, 8, 1, 5, 13, 64, 17465), (F32, 6, 1, 1, 17, 96, 13968), (F32, 8, 9, 2, 49, 96, 17738), (F32, 7, 1, 3, 11, 96, 28560), (F32, 3, 1, 1, 17, 200, 21231),
+        (F32, 7, 1, 3, 11, 200, 7632), (BF16, 8, 9, 3, 11, 16, 14426), (BF16, 8, 1, 1, 17, 16, 22620), (BF16, 8, 9, 5, 26, 16, 10698), (BF16, 8, 1, 5, 13, 16, 23888), (BF16, 7, 1, 3, 11, 64, 20672),
+        (BF16, 5, 1, 1, 17, 64, 26912), (BF16, 8, 9, 3, 43, 64, 28923), (BF16, 6, 1, 5, 13, 64, 25474), (BF16, 7, 1, 1, 17, 96, 22611), (BF16, 7, 1, 3, 11, 96, 11395), (BF16, 8, 9, 5, 27, 96, 27689),
+        (BF16, 7, 1, 5, 13, 96, 18633), (BF16, 6, 1, 1, 17, 200, 25666), (BF16, 6, 1, 3, 11, 200, 3984)]
+
+
+@pytest.mark.parametrize("dtype,seqs,Hkv,group,most,dim,hint", WAYS)
+def test_tree_attention_in_every_way_of_sharing_it_out(ops, dtype, seqs, Hkv, group, most, dim, hint):
+    """A case of every kernel that there is beside the smallest of each width, by the longest cache the call is told; the caches are short and ragged."""
+    rng = random.Random(most * dim)
+    cached, nodes = [rng.choice([0, 1, 63, 64, 65, 130, 257]) for _ in range(seqs)], [most] + [rng.randint(0, 3) for _ in range(seqs - 1)]
+    c = Case(dtype, cached, nodes, Hkv * group, Hkv, dim, rng.choice([1, 8, 16, 24]), seed=most + dim, extra_rows=1)
+    c.check(c.call(ops, c.device(), max_cached=hint))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_tree_attention_rows_that_see_nothing(ops, dtype):
     """Masks of any bits: rows without one and without a cache get zeros, rows without one and with a cache their cache alone."""
