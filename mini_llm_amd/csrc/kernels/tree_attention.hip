@@ -822,8 +822,9 @@ constexpr Way NARROW[] = {{1, 4, 4}, {1, 8, 4}, {1, 8, 2}, {2, 8, 2}, {2, 8, 1}}
 
 // Of every way and number of splits the one whose time is the least by a sum of what was measured, in us: a step (a wavefront's keys of a
 // stage) takes 0.8 and its products, workgroups beyond the compute units take turns, all stages together come at 4.2 TB/s, and a
-// join takes 2.5 and 0.2 a split. The numbers were fitted to 64 calls in all ways of sharing them out: the times taken lie 4% above the best on average
-// where fixed bounds on rows and keys lay 21% above it. Of 174 other calls, drawn later, they lie 3 to 5% above it (55% at most).
+// join takes 6 and 0.2 a split (2.5 of it on the unit's side, the rest the host's: a second launch and a workspace, 14 us a call instead of 11). Over 180 calls
+// in all ways of sharing them out the times taken, the host's among them, lie 3% above the best on average (61% at most); with a join at 2.5 4%, with
+// fixed bounds on rows and keys, over the first 64 of them, 21%.
 Plan plan_of(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_new, int max_cached, int window, int dtype) {
     const bool f32 = dtype == MLLM_F32;
     const int nt = head_dim <= 32 ? 1 : head_dim <= 64 ? 2 : head_dim <= 128 ? 4 : 8, keys = f32 ? 16 : 32;
@@ -843,7 +844,7 @@ Plan plan_of(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_new,
         for (int n = 1; n <= 64 && (n == 1 || (n < 2 * all && groups * n <= 1024)); n += n < 4 ? 1 : n < 8 ? 2 : n < 16 ? 4 : n < 32 ? 8 : 16) {
             const float turns = static_cast<float>((groups * n + 255) / 256), steps = static_cast<float>((all + n - 1) / n);
             const float came = static_cast<float>(groups * n) * steps * w->key_groups * tile_kb * 0.00024f;
-            const float us = 6.5f * (turns - 1) + std::max(turns * steps * step, came) + (n > 1 ? 2.5f + 0.2f * n : 0.f);
+            const float us = 6.5f * (turns - 1) + std::max(turns * steps * step, came) + (n > 1 ? 6.f + 0.2f * n : 0.f);
             if (us < least) {
                 least = us;
                 best = {nt, w->rt, w->waves, w->key_groups, static_cast<int>(row_tiles), n};

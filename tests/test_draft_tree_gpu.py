@@ -250,7 +250,8 @@ WAYS = [(F32, 8, 9, 3, 11, 16, 13500), (F32, 7, 1, 1, 17, 16, 12990), (F32, 8, 9
         (F32, 8, 5, 7, 55, 64, 15668), (F32, 8, 1, 5, 13, 64, 17465), (F32, 6, 1, 1, 17, 96, 13968), (F32, 8, 9, 2, 49, 96, 17738), (F32, 7, 1, 3, 11, 96, 28560), (F32, 3, 1, 1, 17, 200, 21231),
         (F32, 7, 1, 3, 11, 200, 7632), (BF16, 8, 9, 3, 11, 16, 14426), (BF16, 8, 1, 1, 17, 16, 22620), (BF16, 8, 9, 5, 26, 16, 10698), (BF16, 8, 1, 5, 13, 16, 23888), (BF16, 7, 1, 3, 11, 64, 20672),
         (BF16, 5, 1, 1, 17, 64, 26912), (BF16, 8, 9, 3, 43, 64, 28923), (BF16, 6, 1, 5, 13, 64, 25474), (BF16, 7, 1, 1, 17, 96, 22611), (BF16, 7, 1, 3, 11, 96, 11395), (BF16, 8, 9, 5, 27, 96, 27689),
-        (BF16, 7, 1, 5, 13, 96, 18633), (BF16, 6, 1, 1, 17, 200, 25666), (BF16, 6, 1, 3, 11, 200, 3984)]
+        (BF16, 7, 1, 5, 13, 96, 18633), (BF16, 6, 1, 1, 17, 200, 25666), (BF16, 6, 1, 3, 11, 200, 3984),
+        (F32, 8, 5, 7, 55, 16, 28308), (F32, 8, 10, 3, 11, 64, 21717), (BF16, 8, 10, 3, 43, 96, 27944)]
 
 
 @pytest.mark.parametrize("dtype,seqs,Hkv,group,most,dim,hint", WAYS)
