@@ -496,7 +496,7 @@ void glu_act(const Tensor2& gu, int act, const Tensor2& out, hipStream_t stream)
 // parent parents[i] < i within its sequence (-1: a root). step_maps makes the step's arrays, rotary turns queries and keys by its
 // positions, tree_attention reads the cache, and with the token that the model chose at every node tree_accept finds what stands; kv_append
 // then writes the kept nodes' keys and values to the slots it gives. All of it stays on the device, so that the next step can be
-// launched without the host having seen the result of this one.
+// launched without the host having seen the result of this one. A call takes at most 65,536 sequences; outputs lie apart from inputs and each other.
 //
 // rows[b] (null: b): the request's row of lengths, pages (a place without a request: a row outside them). cu_q [n_seqs + 1], cached and
 // ctx_len (cached + new) [n_seqs], token_seq, positions and slots (page rows) [tokens], block_tables [n_seqs, max_blocks] with the pages

@@ -637,7 +637,8 @@ def token_side(x, xb, gate, proj, weight, eps, ids, table, col0, copy=None, next
 # -- trees of drafted tokens -----------------------------------------------------------------------------
 # A step that has the model check several drafted tokens of a request at once: step_maps, (products, rotary, tree_attention) of every
 # layer, argmax or sample at every node, tree_accept, and kv_append with its slots for every layer. A tree is given by its nodes' parents,
-# numbered within the sequence and standing in front of their children; node 0 is the last token that is certain.
+# numbered within the sequence and standing in front of their children; node 0 is the last token that is certain. A call takes at most
+# 65,536 sequences.
 
 def tree_max_nodes() -> int:
     """The most nodes of one sequence's tree."""
