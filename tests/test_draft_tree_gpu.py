@@ -547,6 +547,33 @@ def test_tree_accept_of_one_request_twice(ops):
         assert kept.tolist() == [1] * B
 
 
+def test_the_most_sequences_that_a_call_takes(ops):
+    """65,536 sequences of one node: step maps (portions and trees), attention of nodes that see themselves alone, and paths of one node."""
+    B, page, blocks = 65536, 4, 2
+    n, at = torch.ones(B, dtype=torch.int32, device=DEV), torch.arange(B, dtype=torch.int32, device=DEV)
+    lengths = at % 7
+    pages = torch.stack([at, (at + 1) % B], 1).contiguous()
+    rows = torch.flip(at, [0]).contiguous()
+    for tree in (False, True):
+        m = ops.StepMaps(B, B, blocks, 1, tree=tree)
+        ops.step_maps(m, rows, n, lengths, pages, page, B, torch.full((B,), -1, dtype=torch.int32, device=DEV) if tree else None)
+        want = lengths[rows.long()]
+        assert torch.equal(m.cu_q, torch.arange(B + 1, dtype=torch.int32, device=DEV)) and torch.equal(m.token_seq, at)
+        assert torch.equal(m.cached, want) and torch.equal(m.positions, want) and torch.equal(m.ctx_len, want + 1)
+        if tree:
+            assert (m.slots == -1).all() and (m.ancestors == 1).all()
+        else:
+            assert torch.equal(m.slots, pages[rows.long(), (want // page).long()] * page + want % page)
+    kept, path, following, slots, ends = (torch.full(s, -7, dtype=torch.int32, device=DEV) for s in ((B,), (B, 1), (B,), (B,), (B,)))
+    ops.tree_accept(at, at, torch.full((B,), -1, dtype=torch.int32, device=DEV), m.cu_q, m.cached, m.block_tables, page, B, kept, path, following, slots, ends, rows)
+    assert (kept == 1).all() and torch.equal(path[:, 0], at) and torch.equal(following, at)
+    assert torch.equal(ends[rows.long()], want + 1)
+    q, k, v = (torch.randn(B, 16, device=DEV).to(torch.bfloat16) for _ in range(3))
+    pool, out = torch.randn(B * page, 16, device=DEV).to(torch.bfloat16), torch.zeros(B, 16, dtype=torch.bfloat16, device=DEV)
+    ops.tree_attention(q, k, v, 1, 1, 16, pool, pool, page, m.block_tables, torch.zeros_like(m.cached), m.cu_q, m.ancestors, None, 0.25, out, max_new=1, max_cached=0)
+    assert torch.equal(out, v)
+
+
 def token_by_token(ops, dtype, prompts, steps):
     m = Model(ops, dtype)
     texts, margins = [], []
