@@ -73,7 +73,7 @@ LIBRARIES: Dict[str, dict] = {
     "moe": {"kind": "hip", "sources": ["kernels/moe.hip"], "headers": ["kernels/common.h", "kernels/score_shape.h", "kernels/tanh_norm.h"]},
     "draft_tree": {"kind": "hip", "sources": ["kernels/draft_tree.hip"], "headers": ["kernels/common.h", "kernels/score_shape.h", "kernels/tanh_norm.h"]},
     "rotary": {"kind": "hip", "sources": ["kernels/rotary.hip"], "headers": ["kernels/common.h", "kernels/score_shape.h", "kernels/tanh_norm.h"]},
-    "tree_attention": {"kind": "hip", "sources": ["kernels/tree_attention.hip"], "headers": ["kernels/common.h", "kernels/lds_loads.h", "kernels/score_shape.h", "kernels/tanh_norm.h"]},
+    "tree_attention": {"kind": "hip", "sources": ["kernels/tree_attention.hip"], "headers": ["kernels/common.h", "kernels/lds_loads.h", "kernels/tree_stage.h", "kernels/score_shape.h", "kernels/tanh_norm.h"]},
     "sampling": {"kind": "hip", "sources": ["kernels/sampling.hip"],
                  "headers": ["kernels/common.h", "kernels/score_shape.h", "kernels/tanh_norm.h", "kernels/noalloc.h"]},
     "peaks": {"kind": "hip", "sources": ["kernels/peaks.hip"], "headers": ["kernels/common.h", "kernels/score_shape.h", "kernels/tanh_norm.h"]},

@@ -35,6 +35,7 @@
 // a call out by measured times: 46, 302, 12, 16; values turned by the read: 45, 266, 12, 15.
 #include "common.h"
 #include "lds_loads.h"
+#include "tree_stage.h"
 
 #include <algorithm>
 #include <cmath>
@@ -63,21 +64,6 @@ struct TreeAttentionParams {
     bool negative;
     char* out;
     float* ws;
-};
-
-// Sizes of a kernel for heads of more than 16 NT, up to 32 NT columns (NT = 1: from the first). A row has a power of two of columns in LDS, so that
-// whole rows fill a load instruction; narrower heads leave some of them unused (96 columns as 128: 1.5 times as fast as rows packed without a gap).
-template <typename T, int NT, int KEY_GROUPS_OF_16>
-struct Shape {
-    static constexpr int KT = KEY_GROUPS_OF_16;            // 16-key groups of a tile (bfloat16: a product step of values takes two)
-    static constexpr int KEYS = 16 * KT;
-    static constexpr int CH = NT * sizeof(T) / 2;          // 64-byte pieces of a row
-    static constexpr int PER = 4 / sizeof(T);              // elements of a word
-    static constexpr int TILES = 2 * NT;                   // 16-column tiles of the output
-    static constexpr int LEAST = NT / 2;                   // heads are wider than 32 LEAST
-    static_assert((NT & (NT - 1)) == 0, "a power of two");
-    static constexpr int BLOCK = std::min(CH, 4);          // 32 bits: words of a value row that lie together in a lane
-    static constexpr int WORDS = 4 * KT / PER;             // words of a lane's keys in a column
 };
 
 // Ones (1 in the lowest bit of each element) where a word's elements are not finite. In whole-number arithmetic on all elements of the word at
@@ -304,8 +290,9 @@ struct Rows {
         for (int rt = 0; rt < RT; ++rt) {
             unsigned seen = mine;
             if (of_nodes) {
+                const int word = word_of_nodes(at0, nodes);
                 unsigned long long bits = RT == 1 ? above[rt] : 0;
-                if (RT > 1 || at0 >= 64) bits = a.ancestors[static_cast<size_t>(token[rt]) * a.words + at0 / 64];
+                if (word > 0 || (RT > 1 && word == 0)) bits = a.ancestors[static_cast<size_t>(token[rt]) * a.words + word];
                 bits >>= at0 % 64 + 4 * G;
                 unsigned nodes_seen = 0;
 #pragma unroll
@@ -400,24 +387,6 @@ __device__ __forceinline__ float2* split_state(const TreeAttentionParams& a, siz
 // rows; a 16-byte read of values has eight pieces of a row and the other eight of the row four further on. None meets a bank twice. (By k % 16 alone the
 // reads of values took twice as long, a third of all LDS cycles.)
 constexpr int TABLE_ENTRIES = 2048;
-template <typename T, int NT, int K16, int NW, int KG>
-struct Stage {
-    using S = Shape<T, NT, K16>;
-    static constexpr int ROW = S::CH * 64, PIECES = 4 * S::CH, LEAST = S::KEYS * KG;      // a key group has one tile of a stage at least
-    static constexpr int keys() {          // 24 KB of keys and values at least, in whole instructions of all wavefronts
-        int n = LEAST;
-        while (n * 2 * ROW < 24576 || n * PIECES % (64 * NW) != 0) n *= 2;
-        return n;
-    }
-    static constexpr int KEYS = keys();
-    static constexpr int MATRIX = KEYS * ROW, BYTES = 2 * MATRIX;
-    static constexpr int NUMBER = 4 * BYTES <= 131072 ? 4 : 3;            // one is read, the next has come, the others are on their way
-    static constexpr int LOADS = KEYS * PIECES / 64 / NW;                 // of a wavefront, a stage and matrix
-    static_assert(LOADS * 64 * NW == KEYS * PIECES, "whole instructions");
-    static constexpr int MINE = KEYS / NW, PER_LOAD = 64 / PIECES;        // rows of a wavefront (it loads these), rows of a load instruction
-    static_assert(MINE <= 64 && KEYS % NW == 0, "a bit a row");
-};
-
 template <typename T, int NT, int RT, int K16, int NW, int KG>
 __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionParams a) {
     using R = Rows<T, NT, RT, K16>;
@@ -555,7 +524,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
 
     // One loop over the wavefront's tiles of all stages: in two loops, one in the other, the outputs would be copied from the one's registers
     // to the other's for every tile. (A wavefront whose rows lie behind the last works on the last again, and writes nothing.)
-    constexpr int TURNS = SK / KEYS / KG;
+    constexpr int TURNS = St::TURNS;
     // Everything comes from LDS a phase before it is multiplied: a tile's keys while the tile in front of it is weighed (its stage has come by then),
     // its values while its own products are made.
     constexpr bool SHORT = sizeof(T) == 2;
@@ -870,22 +839,12 @@ int launch(const TreeAttentionParams& p, hipStream_t stream) {
 
 template <typename T>
 int dispatch(const TreeAttentionParams& p, const Plan& plan, hipStream_t stream) {
-    // (16-key groups of a tile: as many as the registers hold beside the outputs where few wavefronts share the keys, so that there is independent
-    // work for the latencies from keys to outputs; where many do, as few as one product takes, so that a stage is not too large)
-    constexpr int ONE = sizeof(T) == 2 ? 2 : 1, TWO = sizeof(T) == 2 ? 4 : 2;
 #define TREE_CASE(N, R, K, W, G) if (plan.nt == N && plan.rt == R && plan.waves == W && plan.key_groups == G) return launch<T, N, R, K, W, G>(p, stream);
-#define TREE_NARROW(N) TREE_CASE(N, 1, ONE, 4, 4) TREE_CASE(N, 1, ONE, 8, 4) TREE_CASE(N, 1, TWO, 8, 2) TREE_CASE(N, 2, ONE, 8, 2) TREE_CASE(N, 2, ONE, 8, 1)
-#define TREE_MIDDLE(N) TREE_CASE(N, 1, ONE, 2, 2) TREE_CASE(N, 1, ONE, 4, 2) TREE_CASE(N, 1, ONE, 8, 2)
-#define TREE_WIDE(N) TREE_CASE(N, 1, ONE, 1, 1) TREE_CASE(N, 1, ONE, 2, 1) TREE_CASE(N, 1, ONE, 4, 1)
-    TREE_NARROW(1) TREE_NARROW(2) TREE_MIDDLE(4) TREE_WIDE(8)
     if constexpr (sizeof(T) == 2) {
-        TREE_CASE(4, 2, ONE, 8, 2) TREE_CASE(4, 2, ONE, 8, 1)
+        TREE_BF16_KERNELS(TREE_CASE)
     } else {
-        TREE_CASE(4, 1, ONE, 8, 1)
+        TREE_F32_KERNELS(TREE_CASE)
     }
-#undef TREE_WIDE
-#undef TREE_MIDDLE
-#undef TREE_NARROW
 #undef TREE_CASE
     return -1;
 }
