@@ -501,7 +501,7 @@ void glu_act(const Tensor2& gu, int act, const Tensor2& out, hipStream_t stream)
 // rows[b] (null: b): the request's row of lengths, pages (a place without a request: a row outside them). cu_q [n_seqs + 1], cached and
 // ctx_len (cached + new) [n_seqs], token_seq, positions and slots (page rows) [tokens], block_tables [n_seqs, max_blocks] with the pages
 // of ctx_len positions and zeros behind them. With parents: positions are cached + depth, slots are -1, and ancestors [tokens, words] has bit i % 64 of
-// word i / 64 set for the node itself and every node above it. A sequence has at most max_new tokens (more are left out), all together
+// word i / 64 set for the node itself and every node above it; without them ancestors may be null, or gets those of a chain. A sequence has at most max_new tokens (more are left out), all together
 // at most `tokens`; the tokens behind the last sequence get sequence 0, position 0, slot -1 and no ancestors.
 struct StepMapsArgs {
     const int *rows = nullptr, *n_new = nullptr, *lengths = nullptr, *pages = nullptr, *parents = nullptr;

@@ -61,7 +61,7 @@ void step_maps(const StepMapsArgs& a, hipStream_t stream) {
         a.token_seq == nullptr || a.positions == nullptr || a.slots == nullptr || a.block_tables == nullptr)
         fail("step_maps: an array is missing");
     if (a.rows == nullptr && a.n_seqs > a.n_requests) fail("step_maps: %d sequences without rows, %d requests", a.n_seqs, a.n_requests);
-    if (a.parents != nullptr) {
+    if (a.parents != nullptr || a.ancestors != nullptr) {
         if (a.max_new > tree_max_nodes()) fail("step_maps: a tree has at most %d nodes, not %d", tree_max_nodes(), a.max_new);
         if (a.ancestors == nullptr || a.words < (a.max_new + 63) / 64 || a.words > tree_max_nodes() / 64)
             fail("step_maps: trees of up to %d nodes need %d words of ancestors a node, not %d", a.max_new, (a.max_new + 63) / 64, a.words);
@@ -69,7 +69,7 @@ void step_maps(const StepMapsArgs& a, hipStream_t stream) {
     need_seqs(a.n_seqs, "step_maps");
     const int64_t n = 4ll * a.n_seqs, t = 4ll * a.tokens;
     need_apart("step_maps", {{"cu_q", a.cu_q, n + 4}, {"cached", a.cached, n}, {"ctx_len", a.ctx_len, n}, {"token_seq", a.token_seq, t}, {"positions", a.positions, t},
-                             {"slots", a.slots, t}, {"block_tables", a.block_tables, n * a.max_blocks}, {"ancestors", a.ancestors, a.parents == nullptr ? 0 : 2 * t * a.words}},
+                             {"slots", a.slots, t}, {"block_tables", a.block_tables, n * a.max_blocks}, {"ancestors", a.ancestors, a.ancestors == nullptr ? 0 : 2 * t * a.words}},
                {{"rows", a.rows, n}, {"n_new", a.n_new, n}, {"lengths", a.lengths, 4ll * a.n_requests},
                 {"pages", a.pages, 4 * ((a.n_requests - 1) * a.ld_pages + a.max_blocks)}, {"parents", a.parents, t}});
     check(mllm_step_maps(a.rows, a.n_new, a.lengths, a.pages, a.ld_pages, a.parents, a.n_seqs, a.n_requests, a.tokens, a.page_size, a.n_pages, a.max_blocks,

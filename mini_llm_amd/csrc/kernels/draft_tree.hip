@@ -90,6 +90,10 @@ __global__ void __launch_bounds__(TREE_THREADS) step_maps_kernel(StepMapsParams 
             a.token_seq[first + i] = b;
             a.positions[first + i] = cached + i;
             a.slots[first + i] = page_row(list, a.max_blocks, a.page_size, a.n_pages, cached + i);
+            for (int w = 0; w < a.words; ++w) {          // (a chain: bits 0 to i)
+                const int bits = i + 1 - 64 * w;
+                a.ancestors[static_cast<size_t>(first + i) * a.words + w] = bits <= 0 ? 0 : bits >= 64 ? ~0ull : (1ull << bits) - 1;
+            }
         }
         return;
     }
@@ -202,16 +206,17 @@ extern "C" {
 
 int mllm_tree_max_nodes(void) { return TREE_MAX_NODES; }
 
-// Returns 0, a HIP error code, or -1 for sizes the kernel refuses. parents null: portions of a text; otherwise trees of at most
-// mllm_tree_max_nodes() nodes, and `ancestors` takes `words` words a token.
+// Returns 0, a HIP error code, or -1 for sizes the kernel refuses. parents null: portions of a text; otherwise trees. Where `ancestors` is not null it
+// takes `words` words a token, of trees and of portions (a chain each), which have at most mllm_tree_max_nodes() nodes then.
 int mllm_step_maps(const int* rows, const int* n_new, const int* lengths, const int* pages, long long ld_pages, const int* parents, int n_seqs,
                    int n_requests, int tokens, int page_size, int n_pages, int max_blocks, int max_new, int words, int* cu_q, int* cached,
                    int* ctx_len, int* token_seq, int* positions, int* slots, int* block_tables, unsigned long long* ancestors, hipStream_t stream) {
     if (n_seqs < 1 || n_requests < 1 || tokens < 1 || page_size < 1 || n_pages < 1 || max_blocks < 1 || max_new < 1) return -1;
     if (static_cast<long long>(n_seqs) * max_new > INT32_MAX || static_cast<long long>(n_pages) * page_size > INT32_MAX) return -1;
-    if (parents != nullptr && (max_new > TREE_MAX_NODES || words < (max_new + 63) / 64 || words > TREE_MAX_NODES / 64)) return -1;
+    if (parents != nullptr && ancestors == nullptr) return -1;
+    if (ancestors != nullptr && (max_new > TREE_MAX_NODES || words < (max_new + 63) / 64 || words > TREE_MAX_NODES / 64)) return -1;
     const StepMapsParams p{rows, n_new, lengths, pages, parents, ld_pages, n_seqs, n_requests, tokens, page_size, n_pages, max_blocks, max_new,
-                           parents != nullptr ? words : 0, cu_q, cached, ctx_len, token_seq, positions, slots, block_tables, ancestors};
+                           ancestors != nullptr ? words : 0, cu_q, cached, ctx_len, token_seq, positions, slots, block_tables, ancestors};
     // (a workgroup for every 1,024 entries of a table or tokens of a portion)
     const int parts = std::min(64, (std::max(max_blocks, parents != nullptr ? 1 : max_new) + 1023) / 1024);
     step_maps_kernel<<<dim3(n_seqs + 1, parts), TREE_THREADS, 0, stream>>>(p);

@@ -749,14 +749,15 @@ def step_maps(maps: StepMaps, rows: Optional[torch.Tensor], n_new: torch.Tensor,
     lengths[r] tokens in the pages pages[r, :] and brings n_new[b] more. All int32: n_new (and rows) [n_seqs], lengths [requests], pages
     [requests, >= max_blocks] (any row stride).
 
-    Without ``parents`` the tokens follow one another: positions from lengths[r] on, slots their page rows. With ``parents`` (int32
+    Without ``parents`` the tokens follow one another: positions from lengths[r] on, slots their page rows (and, in maps made with ``tree=True``,
+    ancestors those of a chain). With ``parents`` (int32
     [tokens], needs maps made with ``tree=True``) they are a tree each: positions are lengths[r] + depth, slots -1 (``tree_accept``
     says later where the kept ones go), ancestors the sets that ``tree_attention`` takes; a parent that does not stand in front of its
     child counts as none. The maps' arrays lie apart from the inputs. More than ``max_new`` tokens of a sequence, or more than ``tokens`` together, are left out (cu_q says how
     many are in). A position beyond ``max_blocks``, or whose page is none of the ``n_pages``, has slot -1. Tokens behind the last sequence get
     sequence 0, position 0, slot -1 and no ancestors."""
     B, T, blocks, mine = maps.n_seqs, maps.tokens, maps.max_blocks, maps.addresses
-    at_new, at_rows, at_parents, words = _counted(n_new, "n_new", B), 0, 0, 0
+    at_new, at_rows, at_parents, words = _counted(n_new, "n_new", B), 0, 0, 0 if maps.ancestors is None else maps.words
     if rows is not None:
         at_rows = _counted(rows, "rows", B)
     _table(pages, "pages")
@@ -767,7 +768,7 @@ def step_maps(maps: StepMaps, rows: Optional[torch.Tensor], n_new: torch.Tensor,
     if parents is not None:
         if maps.ancestors is None:
             raise KernelError("parents need step maps made for trees")
-        at_parents, words = _counted(parents, "parents", T), maps.words
+        at_parents = _counted(parents, "parents", T)
     device = _here(rows, n_new, lengths, pages, parents, maps.cu_q)
     a = _bytes(_MAPS_BYTES, at_rows, at_new, at_lengths, pages.data_ptr(), at_parents, pages.stride(0) if requests > 1 else cols, B, requests, T, page_size,
                n_pages, blocks, maps.max_new, words, *mine)
