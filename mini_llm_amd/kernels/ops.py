@@ -733,14 +733,28 @@ class StepMaps:
         self.token_seq, self.positions, self.slots = zeros(tokens), zeros(tokens), zeros(tokens)
         self.block_tables = zeros(n_seqs, max_blocks)
         self.ancestors = torch.zeros((tokens, self.words), dtype=torch.int64, device=device) if tree else None
+        self._find()
+
+    def _find(self):
         # (the kernel writes to these addresses: the arrays stay the object's own as long as it lives)
         self.addresses = tuple(0 if t is None else t.data_ptr() for t in (self.cu_q, self.cached, self.ctx_len, self.token_seq, self.positions, self.slots,
                                                                           self.block_tables, self.ancestors))
+
+    # (a copy, deep or by way of a file, has arrays of its own and finds them anew)
+    def __getstate__(self):
+        return {name: value for name, value in self.__dict__.items() if name != "addresses"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._find()
 
     def __setattr__(self, name, value):
         if "addresses" in self.__dict__:
             raise AttributeError(f"step maps keep their arrays: copy into '{name}'")
         object.__setattr__(self, name, value)
+
+    def __delattr__(self, name):
+        raise AttributeError(f"step maps keep their arrays, '{name}' among them")
 
 
 def step_maps(maps: StepMaps, rows: Optional[torch.Tensor], n_new: torch.Tensor, lengths: torch.Tensor, pages: torch.Tensor, page_size: int,

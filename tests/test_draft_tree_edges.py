@@ -1,6 +1,8 @@
 """Drafted trees at the edges of what a call allows, without a GPU: which words of a node's ancestors tree attention reads, what maps of
-portions refuse."""
+portions refuse, copies of step maps."""
+import copy
 import os
+import pickle
 import shutil
 import subprocess
 
@@ -31,3 +33,20 @@ def test_ancestors_of_portions_are_checked_as_those_of_trees(change, match):
     """Step maps write the chains' ancestors of portions too, wherever there is an array for them."""
     with pytest.raises(ops.KernelError, match=match):
         native_ints(ops.StepMapsC, "mllm_op_step_maps", MAPS_SIZES, **dict(dict(parents=0), **change))
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("again", [copy.copy, copy.deepcopy, lambda m: pickle.loads(pickle.dumps(m))], ids=["copy", "deepcopy", "pickle"])
+def test_copies_of_step_maps_are_filled_in_their_own_arrays(tree, again):
+    """What the kernel is handed are the addresses of the object's own arrays, not those of the object it was copied from, which may be gone."""
+    maps = ops.StepMaps(2, 8, 3, 4, tree=tree, device="cpu")
+    other = again(maps)
+    names = ("cu_q", "cached", "ctx_len", "token_seq", "positions", "slots", "block_tables", "ancestors")
+    for m in (maps, other):
+        assert m.addresses == tuple(0 if getattr(m, n) is None else getattr(m, n).data_ptr() for n in names)
+    assert (other.addresses == maps.addresses) == (again is copy.copy)          # (a shallow copy shares them)
+    assert [getattr(other, n) for n in ("n_seqs", "tokens", "max_blocks", "max_new", "words")] == [2, 8, 3, 4, 1]
+    with pytest.raises(AttributeError, match="keep their arrays"):
+        other.slots = maps.slots
+    with pytest.raises(AttributeError, match="keep their arrays"):
+        del other.slots
