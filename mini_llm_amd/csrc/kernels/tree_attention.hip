@@ -70,15 +70,17 @@ struct TreeAttentionParams {
 // once: as comparisons, the lanes' answers to all words of a tile fill the scalar registers several times over.
 __device__ __forceinline__ uint32_t not_finite(uint32_t w, float) { return ((w & 0x7f800000u) + 0x00800000u) >> 31; }
 __device__ __forceinline__ uint32_t not_finite(uint32_t w, bf16_t) { return ((w & 0x7f807f80u) + 0x00800080u) >> 15 & 0x00010001u; }
-// kind 0: the elements that are finite, zeros for the others; 1, 2, 3: one where the element is NaN, +inf, -inf, else 0.
+// kind 0: the elements that are finite, zeros for the others; 1, 2, 3, 4: one where the element is NaN, +inf, -inf, any of these, else 0.
 __device__ __forceinline__ uint32_t sifted(uint32_t w, int kind, float) {
     const uint32_t special = not_finite(w, 0.f), mantissa = ((w & 0x7fffffu) + 0x7fffffu) >> 23, sign = w >> 31;
     if (kind == 0) return w & (special - 1);
+    if (kind == 4) return special * 0x3f800000u;
     return (special & (kind == 1 ? mantissa : ~mantissa & (kind == 2 ? ~sign : sign))) * 0x3f800000u;
 }
 __device__ __forceinline__ uint32_t sifted(uint32_t w, int kind, bf16_t) {
     const uint32_t special = not_finite(w, bf16_t{}), mantissa = ((w & 0x007f007fu) + 0x007f007fu) >> 7, sign = w >> 15;
     if (kind == 0) return w & ~(special * 0xffffu);
+    if (kind == 4) return special * 0x3f80u;
     return (special & (kind == 1 ? mantissa : ~mantissa & (kind == 2 ? ~sign : sign))) * 0x3f80u;
 }
 
@@ -278,14 +280,17 @@ struct Rows {
         weigh<false>([&](int j, int w) { return v[w][j]; }, [&](int rt, int j) { return p[rt][j]; },
                      [&](int x, int rt, auto&& product) { o[x][rt] = product(o[x][rt]); }, [&](int rt, auto&& product) { sum[rt] = product(sum[rt]); });
     }
-    // Any tile: keys [at0, at0 + KEYS) of the cache, or of the nodes; `valid` has a bit for each that exists. stored(j, w) gives a word of the values again.
+    // Any tile: keys [at0, at0 + KEYS) of the cache, or of the nodes; `valid` has a bit for each that exists. stored(j, w) gives a word of the values again;
+    // seen_by, the lane's own word of LDS, keeps which of the lane's keys its rows see (a register more all the way does not fit beside 32 rows of 128 columns).
     template <typename W>
     __device__ __forceinline__ void take_some(float (&p)[RT][4 * KT], const uint32_t (&v)[TILES][S::WORDS], const TreeAttentionParams& a, bool of_nodes, int at0,
-                                              unsigned long long valid, int first, int nodes, W&& stored) {
+                                              unsigned long long valid, int first, int nodes, unsigned* seen_by, W&& stored) {
         const int G = threadIdx.x % 64 / 16;
         unsigned mine = 0;                   // which of the lane's keys exist
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) mine |= static_cast<unsigned>(valid >> (16 * kt + 4 * G) & 15) << (4 * kt);
+        static_assert(RT * 4 * KT <= 32, "a bit a row and key");
+        unsigned all_seen = 0;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             unsigned seen = mine;
@@ -308,11 +313,14 @@ struct Rows {
                 }
 #pragma unroll
             for (int j = 0; j < 4 * KT; ++j) p[rt][j] = seen >> j & 1 ? p[rt][j] : -INFINITY;
+            all_seen |= seen << (4 * KT * rt);
         }
+        *seen_by = all_seen;
         weights(p, a.scale);
         // A key that does not exist has some other row's values. A value that is not finite, in a tile of which some rows see less than others,
         // would reach those that do not see it as zero times it: the finite values are weighed as ever, and whether a row gives weight to a NaN,
-        // +inf or -inf of a column is a product of ones and zeros. (For these products the words are read anew, which keeps them out of the registers.)
+        // +inf or -inf of a column, or sees any of these and gives it none (zero times it, NaN, as where all rows see all keys), is a product of ones and
+        // zeros. (For these products the words are read anew, which keeps them out of the registers.)
         auto exists = [&](int j) {           // (of the keys of word j)
             return sizeof(T) == 2 ? (mine >> 2 * j & 1 ? 0xffffu : 0u) | (mine >> 2 * j & 2 ? 0xffff0000u : 0u) : 0u - (mine >> j & 1);
         };
@@ -335,17 +343,24 @@ struct Rows {
         }
         auto word = [&](int j, int w) { return stored(j, w) & exists(j); };
         weigh<true>([&](int j, int w) { return sifted(word(j, w), 0, T{}); }, weight, add, added);
+        auto to_those = [&](float value) {
+            return [this, value](int x, int rt, auto&& product) {
+                const f32x4 count = product(f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[x][rt][i] += count[i] > 0.f ? value : 0.f;
+            };
+        };
+        auto no_sum = [](int, auto&&) {};
 #pragma unroll 1
         for (int kind = 1; kind <= 3; ++kind) {
-            const float value = kind == 1 ? __builtin_nanf("") : kind == 2 ? INFINITY : -INFINITY;
             asm volatile("" ::: "memory");
             weigh<true>([&](int j, int w) { return sifted(word(j, w), kind, T{}); }, [&](int rt, int j) { return p[rt][j] == 0.f ? 0.f : 1.f; },
-                        [&](int x, int rt, auto&& product) {
-                            const f32x4 count = product(f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) o[x][rt][i] += count[i] > 0.f ? value : 0.f;
-                        }, [](int, auto&&) {});
+                        to_those(kind == 1 ? __builtin_nanf("") : kind == 2 ? INFINITY : -INFINITY), no_sum);
         }
+        asm volatile("" ::: "memory");
+        const unsigned seen = *seen_by;
+        weigh<true>([&](int j, int w) { return sifted(word(j, w), 4, T{}); },
+                    [&](int rt, int j) { return p[rt][j] == 0.f && seen >> (4 * KT * rt + j) & 1 ? 1.f : 0.f; }, to_those(__builtin_nanf("")), no_sum);
     }
 
     // o[x][rt][i] stands in column column(x) + EACH (4 G + i) of its row.
@@ -400,6 +415,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
     // the stages [keys, values][SK][PIECES * 16]; at the end the states [wavefront][16 RT][PITCH], then their maxima and sums
     extern __shared__ __attribute__((aligned(512))) unsigned char stage_s[];
     __shared__ int table_s[TABLE_ENTRIES];
+    __shared__ unsigned seen_s[NW * 64];                                  // of each lane
     __shared__ unsigned long long valid_s[St::NUMBER][NW];                // of each wavefront's rows of a stage: a bit a key that exists
     Work w;
     if (!w.find(a, 16 * RT * RG)) return;
@@ -633,7 +649,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             }
             some = static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(some >> 32)))) << 32 |
                    static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(some)));
-            r.take_some(p, v, a, of_nodes, at0 + k0, some, first, nodes, [&](int j, int x) {
+            r.take_some(p, v, a, of_nodes, at0 + k0, some, first, nodes, seen_s + threadIdx.x, [&](int j, int x) {
                 if constexpr (SHORT) {
                     const u32x2 u = two_words(keys, j / 2, x);
                     return j % 2 == 0 ? u.x : u.y;
@@ -829,7 +845,7 @@ int launch(const TreeAttentionParams& p, hipStream_t stream) {
     const long long blocks = (static_cast<long long>(p.units) + 7) / 8 * 8 * p.row_tiles;
     if (blocks * NW * 64 > UINT32_MAX) return -1;          // (what one launch can have)
     constexpr int STATES = KG == 1 ? 0 : NW * 16 * RT * ((32 * NT + 4) * 4 + 8), LDS = std::max(St::NUMBER * St::BYTES, STATES);
-    static_assert(LDS + TABLE_ENTRIES * 4 + 1024 <= 163840, "LDS of a compute unit");
+    static_assert(LDS + TABLE_ENTRIES * 4 + NW * 256 + 1024 <= 163840, "LDS of a compute unit");
     auto kernel = tree_attention_kernel<T, NT, RT, K16, NW, KG>;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (e != hipSuccess) return static_cast<int>(e);

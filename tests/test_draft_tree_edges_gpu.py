@@ -1,12 +1,18 @@
-"""Drafted trees at the edges of what a call allows, against the plain implementations in 64 bits (tests/plain_tree.py)."""
+"""Drafted trees at the edges of what a call allows: maps used for trees and portions in turn, values that are not finite; against the plain implementations in 64
+bits (tests/plain_tree.py)."""
+import math
 import random
 
 import pytest
+import torch
 
 import plain_tree
-from test_draft_tree_gpu import ints, ops, random_tree  # noqa: F401
+from test_draft_tree_gpu import DEV, DTYPES, WAYS, Case, ints, ops, random_tree  # noqa: F401
 
 pytestmark = pytest.mark.gpu
+
+LN2 = math.log(2.0)        # as the scale: scores are powers of two
+
 
 # -- step maps ----------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("most", [1, 5, 64, 65, 130, 256])
@@ -28,3 +34,50 @@ def test_step_maps_of_portions_in_maps_made_for_trees(ops, most):  # noqa: F811
             want["ancestors"] = plain_tree.step_maps(rows, n_new, lengths, pages, page, 50, tokens, blocks, most, chain)["ancestors"]
         for name, value in want.items():
             assert getattr(maps, name).tolist() == value, name
+
+
+# -- attention ----------------------------------------------------------------------------------------------------------------
+def one_column_case(dtype, cached, nodes, H, Hkv, dim, page, **more):
+    """Scores are the keys' first column in powers of two: all zero at first."""
+    c = Case(dtype, cached, nodes, H, Hkv, dim, page, scale=LN2, **more)
+    kv = Hkv * dim
+    c.qkv[:, :-2 * kv] = 0.0
+    c.qkv[:, 0:H * dim:dim] = 1.0
+    c.qkv[:, H * dim:H * dim + kv:dim] = 0.0
+    c.k_pages[:, 0:kv:dim] = 0.0
+    return c
+
+
+def way_case(dtype, seqs, Hkv, group, most, dim):
+    rng = random.Random(most * dim + seqs)
+    cached, nodes = [rng.choice([0, 1, 63, 64, 130, 257, 600]) for _ in range(seqs)], [most] + [rng.randint(0, 3) for _ in range(seqs - 1)]
+    return one_column_case(dtype, cached, nodes, Hkv * group, Hkv, dim, rng.choice([1, 7, 16, 64]), seed=most + dim, extra_rows=1)
+
+
+def same_with_what_is_not_finite(c, got):
+    want, bound = c.want()
+    rows = c.cu_q[-1]
+    got = got.double().cpu()[:rows]
+    want, bound = want[:rows], bound[:rows]
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    odd = torch.isinf(want) | torch.isinf(got)
+    assert torch.equal(got[odd], want[odd])
+    plain = torch.isfinite(want)
+    assert ((got - want).abs()[plain] <= bound[plain]).all()
+    return want
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype,seqs,Hkv,group,most,dim,hint", WAYS)
+def test_tree_attention_of_a_seen_value_that_is_not_finite_and_weighs_nothing(ops, dtype, seqs, Hkv, group, most, dim, hint, value):  # noqa: F811
+    """Zero times infinity wherever the key lies: in a tile that all rows see in full or one of pages, nodes or ends that they do not."""
+    c = way_case(dtype, seqs, Hkv, group, most, dim)
+    for b in range(seqs):
+        key, column = (slice(c.H * dim, c.H * dim + Hkv * dim, dim), slice(c.H * dim + Hkv * dim + 1, None, dim)), slice(1, None, dim)
+        for at in {0, c.cached[b] // 2, c.cached[b] - 1} if c.cached[b] > 0 and b % 2 == 0 else ():
+            row = c.tables[b][at // c.page] * c.page + at % c.page
+            c.k_pages[row, 0::dim], c.v_pages[row, column] = -4096.0, value
+        if c.nodes[b] > 0 and b % 2 == 1:
+            c.qkv[c.cu_q[b], key[0]], c.qkv[c.cu_q[b], key[1]] = -4096.0, value
+    want = same_with_what_is_not_finite(c, c.call(ops, c.device(), max_cached=hint))
+    assert torch.isnan(want[:, 1]).any() and torch.isfinite(want[:, 0]).all()
