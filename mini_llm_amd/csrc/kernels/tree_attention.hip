@@ -235,9 +235,9 @@ struct Rows {
             }
         }
     }
-    // Products to weights 2^(scale p - m), scale > 0 (what is not seen is -inf). The maximum that weights are taken against follows only when
-    // a product lies 8 above it: weights then reach 2^8, which costs no accuracy, and most tiles leave sums and outputs as they are and
-    // need not know the maximum over a row's four lanes.
+    // Products to weights 2^(scale p - m), scale > 0 (what is not seen is -inf). What weights are taken against is put 8 above the maximum, and follows
+    // only when a product lies above it: the largest weight then lies between 2^-8 and 1, which costs no accuracy, and most tiles leave sums and outputs as
+    // they are and need not know the maximum over a row's four lanes. (No weight is above 1, so that values add up as far as they would by the maximum itself.)
     __device__ __forceinline__ void weights(float (&p)[RT][4 * KT], float scale) {
         float mx[RT];
         bool any = false;
@@ -247,15 +247,15 @@ struct Rows {
 #pragma unroll
             for (int j = 1; j < 4 * KT; ++j) mx[rt] = fmaxf(mx[rt], p[rt][j]);
             mx[rt] *= scale;
-            any |= mx[rt] > m[rt] + 8.f;
+            any |= mx[rt] > m[rt];
         }
         if (__any(any))
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 const float top = rows_max(mx[rt]);
-                const bool more = top > m[rt] + 8.f;
-                const float fix = more ? exp2_for<T>(m[rt] - top) : 1.f;
-                m[rt] = more ? top : m[rt];
+                const bool more = top > m[rt];
+                const float fix = more ? exp2_for<T>(m[rt] - (top + 8.f)) : 1.f;
+                m[rt] = more ? top + 8.f : m[rt];
                 sum[rt] *= fix;
 #pragma unroll
                 for (int x = 0; x < TILES; ++x) o[x][rt] *= fix;

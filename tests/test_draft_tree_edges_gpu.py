@@ -1,5 +1,5 @@
-"""Drafted trees at the edges of what a call allows: maps used for trees and portions in turn, values that are not finite; against the plain implementations in 64
-bits (tests/plain_tree.py)."""
+"""Drafted trees at the edges of what a call allows: maps used for trees and portions in turn, values that are not finite or next to it; against the plain
+implementations in 64 bits (tests/plain_tree.py)."""
 import math
 import random
 
@@ -81,3 +81,16 @@ def test_tree_attention_of_a_seen_value_that_is_not_finite_and_weighs_nothing(op
             c.qkv[c.cu_q[b], key[0]], c.qkv[c.cu_q[b], key[1]] = -4096.0, value
     want = same_with_what_is_not_finite(c, c.call(ops, c.device(), max_cached=hint))
     assert torch.isnan(want[:, 1]).any() and torch.isfinite(want[:, 0]).all()
+
+
+@pytest.mark.parametrize("dtype,seqs,Hkv,group,most,dim,hint", WAYS)
+def test_tree_attention_of_large_values_whose_keys_come_late(ops, dtype, seqs, Hkv, group, most, dim, hint):  # noqa: F811
+    """The nodes' scores lie 7 (in powers of two) above those of the cache, the values of some nodes at a tenth of the largest number: what is added up stays below the
+    type's largest, as with weights of at most one."""
+    c = way_case(dtype, seqs, Hkv, group, most, dim)
+    kv = Hkv * dim
+    c.qkv[:, c.H * dim:c.H * dim + kv:dim] = 7.0
+    for b in range(seqs):
+        if c.nodes[b] > 0:
+            c.qkv[c.cu_q[b], -kv:] = 3e37 * c.qkv[c.cu_q[b], -kv:].sign()
+    c.check(c.call(ops, c.device(), max_cached=hint))
