@@ -70,18 +70,17 @@ struct TreeAttentionParams {
 // once: as comparisons, the lanes' answers to all words of a tile fill the scalar registers several times over.
 __device__ __forceinline__ uint32_t not_finite(uint32_t w, float) { return ((w & 0x7f800000u) + 0x00800000u) >> 31; }
 __device__ __forceinline__ uint32_t not_finite(uint32_t w, bf16_t) { return ((w & 0x7f807f80u) + 0x00800080u) >> 15 & 0x00010001u; }
-// kind 0: the elements that are finite, zeros for the others; 1, 2, 3, 4: one where the element is NaN, +inf, -inf, any of these, else 0.
-__device__ __forceinline__ uint32_t sifted(uint32_t w, int kind, float) {
-    const uint32_t special = not_finite(w, 0.f), mantissa = ((w & 0x7fffffu) + 0x7fffffu) >> 23, sign = w >> 31;
-    if (kind == 0) return w & (special - 1);
-    if (kind == 4) return special * 0x3f800000u;
-    return (special & (kind == 1 ? mantissa : ~mantissa & (kind == 2 ? ~sign : sign))) * 0x3f800000u;
+// The elements that are finite, zeros for the others.
+__device__ __forceinline__ uint32_t finite(uint32_t w, float) { return w & (not_finite(w, 0.f) - 1); }
+__device__ __forceinline__ uint32_t finite(uint32_t w, bf16_t) { return w & ~(not_finite(w, bf16_t{}) * 0xffffu); }
+// 1 where the element is NaN, 2^7 for +inf, 2^14 for -inf, else 0: sums of up to 127 of them tell how many of each there were.
+__device__ __forceinline__ uint32_t counted(uint32_t w, float) {
+    const uint32_t special = not_finite(w, 0.f), nan = ((w & 0x7fffffu) + 0x7fffffu) >> 23;
+    return special * (0x3f800000u + (1 - nan) * (0x03800000u << (w >> 31)));
 }
-__device__ __forceinline__ uint32_t sifted(uint32_t w, int kind, bf16_t) {
-    const uint32_t special = not_finite(w, bf16_t{}), mantissa = ((w & 0x007f007fu) + 0x007f007fu) >> 7, sign = w >> 15;
-    if (kind == 0) return w & ~(special * 0xffffu);
-    if (kind == 4) return special * 0x3f80u;
-    return (special & (kind == 1 ? mantissa : ~mantissa & (kind == 2 ? ~sign : sign))) * 0x3f80u;
+__device__ __forceinline__ uint32_t counted(uint32_t w, bf16_t) {
+    const uint32_t special = not_finite(w, bf16_t{}), inf = special & ~(((w & 0x007f007fu) + 0x007f007fu) >> 7);
+    return special * 0x3f80u + (inf + (inf & w >> 15)) * 0x0380u;
 }
 
 // What a row's weights are taken against before it has seen a key: finite, so that no difference of two of them is NaN.
@@ -318,9 +317,9 @@ struct Rows {
         *seen_by = all_seen;
         weights(p, a.scale);
         // A key that does not exist has some other row's values. A value that is not finite, in a tile of which some rows see less than others,
-        // would reach those that do not see it as zero times it: the finite values are weighed as ever, and whether a row gives weight to a NaN,
-        // +inf or -inf of a column, or sees any of these and gives it none (zero times it, NaN, as where all rows see all keys), is a product of ones and
-        // zeros. (For these products the words are read anew, which keeps them out of the registers.)
+        // would reach those that do not see it as zero times it: the finite values are weighed as ever, and how many NaN, +inf and -inf a row gives weight
+        // to in a column, and whether it sees any of these and gives it none (zero times it: NaN, as where all rows see all keys), comes out of a product of their
+        // marks with ones, and 2^21 for the keys of the last kind. (For these products the words are read anew, which keeps them out of the registers.)
         auto exists = [&](int j) {           // (of the keys of word j)
             return sizeof(T) == 2 ? (mine >> 2 * j & 1 ? 0xffffu : 0u) | (mine >> 2 * j & 2 ? 0xffff0000u : 0u) : 0u - (mine >> j & 1);
         };
@@ -342,25 +341,20 @@ struct Rows {
             return;
         }
         auto word = [&](int j, int w) { return stored(j, w) & exists(j); };
-        weigh<true>([&](int j, int w) { return sifted(word(j, w), 0, T{}); }, weight, add, added);
-        auto to_those = [&](float value) {
-            return [this, value](int x, int rt, auto&& product) {
-                const f32x4 count = product(f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[x][rt][i] += count[i] > 0.f ? value : 0.f;
-            };
-        };
-        auto no_sum = [](int, auto&&) {};
-#pragma unroll 1
-        for (int kind = 1; kind <= 3; ++kind) {
-            asm volatile("" ::: "memory");
-            weigh<true>([&](int j, int w) { return sifted(word(j, w), kind, T{}); }, [&](int rt, int j) { return p[rt][j] == 0.f ? 0.f : 1.f; },
-                        to_those(kind == 1 ? __builtin_nanf("") : kind == 2 ? INFINITY : -INFINITY), no_sum);
-        }
+        weigh<true>([&](int j, int w) { return finite(word(j, w), T{}); }, weight, add, added);
         asm volatile("" ::: "memory");
+        static_assert(KEYS <= 127, "as many marks");
         const unsigned seen = *seen_by;
-        weigh<true>([&](int j, int w) { return sifted(word(j, w), 4, T{}); },
-                    [&](int rt, int j) { return p[rt][j] == 0.f && seen >> (4 * KT * rt + j) & 1 ? 1.f : 0.f; }, to_those(__builtin_nanf("")), no_sum);
+        weigh<true>([&](int j, int w) { return counted(word(j, w), T{}); }, [&](int rt, int j) { return p[rt][j] != 0.f ? 1.f : seen >> (4 * KT * rt + j) & 1 ? 2097152.f : 0.f; },
+                    [&](int x, int rt, auto&& product) {
+                        const f32x4 marks = product(f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int n = static_cast<int>(fminf(marks[i], 4194304.f));
+                            const float up = n & 0x3f80 ? INFINITY : 0.f, down = n & 0x1fc000 ? -INFINITY : 0.f;
+                            o[x][rt][i] += n & 127 || n >= 1 << 21 ? __builtin_nanf("") : up + down;
+                        }
+                    }, [](int, auto&&) {});
     }
 
     // o[x][rt][i] stands in column column(x) + EACH (4 G + i) of its row.
