@@ -38,6 +38,7 @@
 #include "tree_stage.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -83,8 +84,8 @@ __device__ __forceinline__ uint32_t counted(uint32_t w, bf16_t) {
     return special * 0x3f80u + (inf + (inf & w >> 15)) * 0x0380u;
 }
 
-// What a row's weights are taken against before it has seen a key: finite, so that no difference of two of them is NaN.
-constexpr float LEAST_SCORE = -3.0e38f;
+// What a row's weights are taken against before it has seen a key: finite, so that no difference of two of them is NaN, and no finite score is below it.
+constexpr float LEAST_SCORE = -FLT_MAX;
 
 // a / b for 0 <= a < 2^20, 1 <= b < 2^20, by the reciprocal: half a unit more than `a` lies further from the next quotient than it errs.
 __device__ __forceinline__ int lane_quotient(int a, int b) { return static_cast<int>((static_cast<float>(a) + 0.5f) * __builtin_amdgcn_rcpf(static_cast<float>(b))); }
@@ -362,6 +363,10 @@ struct Rows {
     __device__ __forceinline__ static constexpr int column(int x) { return x / EACH * 16 * EACH + x % EACH; }
 };
 
+__device__ __forceinline__ int cached_of(const TreeAttentionParams& a, int b) {
+    return static_cast<int>(min(min(static_cast<long long>(max(a.cached[b], 0)), static_cast<long long>(a.max_blocks) * a.page_size), INT32_MAX - 65536ll));
+}
+
 // What a workgroup works on, the same in all its threads.
 struct Work {
     int b, hk, split, row_tile, group, first, nodes, rows, cached;
@@ -379,13 +384,30 @@ struct Work {
         first = min(max(a.cu_q[b], 0), a.tokens);
         nodes = min(min(max(a.cu_q[b + 1] - first, 0), a.tokens - first), a.max_new);
         rows = nodes * group;
-        cached = static_cast<int>(min(min(static_cast<long long>(max(a.cached[b], 0)), static_cast<long long>(a.max_blocks) * a.page_size), INT32_MAX - 65536ll));
+        cached = cached_of(a, b);
         return row_tile * rows_each < rows;
     }
 };
 
 __device__ __forceinline__ int block_of(const TreeAttentionParams& a, int at) {
     return static_cast<int>((static_cast<unsigned long long>(static_cast<unsigned>(at)) * a.page_magic) >> a.page_shift);
+}
+// The factor of a row whose weights add up to zero: zero if it sees nothing; else all that it sees scores -inf, no weights can be found, and it is NaN. (What it takes
+// is read anew from the arguments, which are all that either kernel has: kept in scalar registers from the start it costs every call 0.2 us.)
+__device__ __forceinline__ float factor_of_none(int b, int t) {
+    auto at = reinterpret_cast<uintptr_t>(__builtin_amdgcn_kernarg_segment_ptr());
+    asm volatile("" : "+s"(at));
+    const auto& a = *reinterpret_cast<const TreeAttentionParams*>(at);
+    const int first = min(max(a.cu_q[b], 0), a.tokens), nodes = min(min(max(a.cu_q[b + 1] - first, 0), a.tokens - first), a.max_new), cached = cached_of(a, b);
+    const int low = a.window > 0 ? a.positions[t] - a.window + 1 : 0;
+#pragma unroll 1
+    for (int i = 0; i < nodes; ++i)
+        if (a.ancestors[static_cast<size_t>(t) * a.words + i / 64] >> i % 64 & 1 && (a.window <= 0 || a.positions[first + i] >= low)) return __builtin_nanf("");
+    if (low < cached)
+#pragma unroll 1
+        for (int block = max(low, 0) / a.page_size; static_cast<long long>(block) * a.page_size < cached; ++block)
+            if (static_cast<unsigned>(a.block_tables[static_cast<size_t>(b) * a.max_blocks + block]) < static_cast<unsigned>(a.n_pages)) return __builtin_nanf("");
+    return 0.f;
 }
 __device__ __forceinline__ float2* split_state(const TreeAttentionParams& a, size_t pair) {
     return reinterpret_cast<float2*>(a.ws + static_cast<size_t>(a.tokens) * a.n_heads * a.nsplit * a.head_dim) + pair;
@@ -661,7 +683,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             const float sum = r.sum_of(rt);
             if (row >= w.rows) continue;
             const int node = row / w.group, t = first + node, h = hk * w.group + row - node * w.group;
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const float inv = a.nsplit > 1 ? 1.f : sum == 0.f ? factor_of_none(w.b, t) : 1.f / sum;
             T* to = reinterpret_cast<T*>(a.out + t * a.ldo) + h * a.head_dim;
             const size_t pair = (static_cast<size_t>(t) * a.n_heads + h) * a.nsplit + w.split;
             float* part = a.ws + pair * a.head_dim;
@@ -730,7 +752,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
         }
         const int node = (group0 + row) / w.group, t = first + node, h = hk * w.group + group0 + row - node * w.group;
         if (a.nsplit == 1) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const float inv = sum == 0.f ? factor_of_none(w.b, t) : 1.f / sum;
             T* to = reinterpret_cast<T*>(a.out + t * a.ldo) + h * a.head_dim + d;
 #pragma unroll
             for (int e = 0; e < 4; ++e) to[e] = from_float<T>(v[e] * inv);
@@ -781,7 +803,7 @@ __global__ void __launch_bounds__(256) tree_attention_join_kernel(TreeAttentionP
                 for (int j = 0; j < 4; ++j) v[j] += counts ? weight * part[i][j] : 0.f;
             }
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float inv = sum == 0.f ? factor_of_none(b, t) : 1.f / sum;
         T* to = reinterpret_cast<T*>(a.out + t * a.ldo) + h * a.head_dim + d;
 #pragma unroll
         for (int i = 0; i < 4; ++i) to[i] = from_float<T>(v[i] * inv);

@@ -1,5 +1,5 @@
-"""Drafted trees at the edges of what a call allows: maps used for trees and portions in turn, values that are not finite or next to it; against the plain
-implementations in 64 bits (tests/plain_tree.py)."""
+"""Drafted trees at the edges of what a call allows: maps used for trees and portions in turn, values and scores that are not finite or next to it; against the
+plain implementations in 64 bits (tests/plain_tree.py)."""
 import math
 import random
 
@@ -94,3 +94,35 @@ def test_tree_attention_of_large_values_whose_keys_come_late(ops, dtype, seqs, H
         if c.nodes[b] > 0:
             c.qkv[c.cu_q[b], -kv:] = 3e37 * c.qkv[c.cu_q[b], -kv:].sign()
     c.check(c.call(ops, c.device(), max_cached=hint))
+
+
+@pytest.mark.parametrize("dtype,seqs,Hkv,group,most,dim,hint", WAYS)
+def test_tree_attention_of_keys_that_all_score_minus_infinity(ops, dtype, seqs, Hkv, group, most, dim, hint):  # noqa: F811
+    """No weights can be found: NaN, as the formula has it; zeros are for rows that see nothing."""
+    c = way_case(dtype, seqs, Hkv, group, most, dim)
+    c.qkv[:, c.H * dim:c.H * dim + Hkv * dim:dim] = -math.inf
+    c.k_pages[:, 0::dim] = -math.inf
+    rng = random.Random(most)
+    c.ancestors = [[0] * c.words if rng.random() < 0.4 else a for a in c.ancestors]
+    for b in range(seqs):                 # (one sequence's pages are none, and a cache of one finite key)
+        if b % 4 == 1:
+            c.tables[b] = [-1] * len(c.tables[b])
+        if b % 4 == 2 and c.cached[b] > 0:
+            at = c.cached[b] // 3
+            c.k_pages[c.tables[b][at // c.page] * c.page + at % c.page, 0::dim] = 3.0
+    same_with_what_is_not_finite(c, c.call(ops, c.device(), max_cached=hint))
+    c.window, c.positions = 5, [p + 3 for p in c.positions]
+    same_with_what_is_not_finite(c, c.call(ops, c.device(), max_cached=hint))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tree_attention_of_scores_next_to_the_least_number(ops, dtype):  # noqa: F811
+    """Finite scores below all that a running maximum may begin with."""
+    c = one_column_case(dtype, [40, 0], [6, 5], 2, 1, 32, 8, seed=3)
+    c.qkv[:, 64:96:32] = -3.3e38
+    c.k_pages[:, 0::32] = -3.3e38
+    # (the scores are equal, so that the result is the mean of the values; their products' own error is as large as they are)
+    got = c.call(ops, c.device()).double().cpu()
+    c.qkv[:, 64:96:32], c.k_pages[:, 0::32] = 0.0, 0.0
+    want, bound = c.want()
+    assert ((got - want).abs() <= bound)[:11].all()
