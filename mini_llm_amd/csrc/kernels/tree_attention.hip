@@ -90,6 +90,9 @@ constexpr float LEAST_SCORE = -FLT_MAX;
 // a / b for 0 <= a < 2^20, 1 <= b < 2^20, by the reciprocal: half a unit more than `a` lies further from the next quotient than it errs.
 __device__ __forceinline__ int lane_quotient(int a, int b) { return static_cast<int>((static_cast<float>(a) + 0.5f) * __builtin_amdgcn_rcpf(static_cast<float>(b))); }
 
+// The first position that a row at `position` sees through a window, or the least number if that lies below it.
+__device__ __forceinline__ int low_of(int position, int window) { return max(position, INT32_MIN + window) - window + 1; }
+
 // One wavefront's rows, 16 RT of them, and what it has summed up for them.
 template <typename T, int NT, int RT, int KEY_GROUPS_OF_16>
 struct Rows {
@@ -121,7 +124,7 @@ struct Rows {
                 q[rt][c] = *reinterpret_cast<const uint4*>(at + (off < row_bytes ? off : 0));
             }
             if (RT == 1) above[rt] = a.ancestors[static_cast<size_t>(token[rt]) * a.words];
-            low[rt] = a.window > 0 ? a.positions[token[rt]] - a.window + 1 : INT32_MIN;
+            low[rt] = a.window > 0 ? low_of(a.positions[token[rt]], a.window) : INT32_MIN;
             low_least = min(low_least, low[rt]);
             low_most = max(low_most, low[rt]);
         }
@@ -399,7 +402,7 @@ __device__ __forceinline__ float factor_of_none(int b, int t) {
     asm volatile("" : "+s"(at));
     const auto& a = *reinterpret_cast<const TreeAttentionParams*>(at);
     const int first = min(max(a.cu_q[b], 0), a.tokens), nodes = min(min(max(a.cu_q[b + 1] - first, 0), a.tokens - first), a.max_new), cached = cached_of(a, b);
-    const int low = a.window > 0 ? a.positions[t] - a.window + 1 : 0;
+    const int low = a.window > 0 ? low_of(a.positions[t], a.window) : 0;
 #pragma unroll 1
     for (int i = 0; i < nodes; ++i)
         if (a.ancestors[static_cast<size_t>(t) * a.words + i / 64] >> i % 64 & 1 && (a.window <= 0 || a.positions[first + i] >= low)) return __builtin_nanf("");
@@ -468,7 +471,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
         if (lane == 0) table_s[wave] = least;
         __syncthreads();
         for (int i = 0; i < NW; ++i) least = min(least, table_s[i]);
-        first_tile = __builtin_amdgcn_readfirstlane(min(max(least - a.window + 1, 0), cached) / SK);
+        first_tile = __builtin_amdgcn_readfirstlane(min(max(low_of(least, a.window), 0), cached) / SK);
     }
     const int cache_tiles = (cached + SK - 1) / SK - first_tile, all_tiles = cache_tiles + (nodes + SK - 1) / SK;
     const int per = (all_tiles + a.nsplit - 1) / a.nsplit, begin = w.split * per, end = min(all_tiles, begin + per);

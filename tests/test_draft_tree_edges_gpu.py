@@ -1,5 +1,5 @@
-"""Drafted trees at the edges of what a call allows: maps used for trees and portions in turn, values and scores that are not finite or next to it; against the
-plain implementations in 64 bits (tests/plain_tree.py)."""
+"""Drafted trees at the edges of what a call allows: maps used for trees and portions in turn, values and scores that are not finite or next to it, positions and
+lengths below zero; against the plain implementations in 64 bits (tests/plain_tree.py)."""
 import math
 import random
 
@@ -126,3 +126,10 @@ def test_tree_attention_of_scores_next_to_the_least_number(ops, dtype):  # noqa:
     c.qkv[:, 64:96:32], c.k_pages[:, 0::32] = 0.0, 0.0
     want, bound = c.want()
     assert ((got - want).abs() <= bound)[:11].all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tree_attention_of_positions_below_zero_and_the_widest_window(ops, dtype):  # noqa: F811
+    c = Case(dtype, [100, 30], [9, 20], 4, 2, 64, 16, seed=5, window=2 ** 31 - 1)
+    c.positions = [p - 200 for p in c.positions]
+    c.check(c.call(ops, c.device()))
