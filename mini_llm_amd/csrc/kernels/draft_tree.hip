@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(TREE_THREADS) tree_accept_kernel(TreeAcceptPar
         return;
     }
     const int all = min(max(a.cu_q[b + 1] - first, 0), a.tokens - first), n = min(all, a.max_new);
-    const int cached = a.cached[b];
+    const int cached = min(max(a.cached[b], 0), INT32_MAX - a.max_new);
     int id = 0, parent = -1, child = NONE, place = -1;
     if (tid < n) {
         id = a.ids[first + tid];

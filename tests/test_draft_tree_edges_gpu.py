@@ -133,3 +133,22 @@ def test_tree_attention_of_positions_below_zero_and_the_widest_window(ops, dtype
     c = Case(dtype, [100, 30], [9, 20], 4, 2, 64, 16, seed=5, window=2 ** 31 - 1)
     c.positions = [p - 200 for p in c.positions]
     c.check(c.call(ops, c.device()))
+
+
+# -- acceptance ---------------------------------------------------------------------------------------------------------------
+def accept(ops, choices, ids, parents, cu_q, cached, tables, page, n_pages, most, lengths, rows=None):  # noqa: F811
+    B, T = len(cached), len(choices)
+    kept, following, slots, path = ints([9] * B), ints([9] * B), ints([9] * T), torch.full((B, most), 9, dtype=torch.int32, device=DEV)
+    ops.tree_accept(ints(choices), ints(ids), ints(parents), ints(cu_q), ints(cached), ints(tables), page, n_pages, kept, path, following, slots, lengths=lengths,
+                    rows=None if rows is None else ints(rows))
+    return [x.tolist() for x in (kept, path, following, slots)]
+
+
+def test_tree_accept_takes_lengths_that_are_none_as_none(ops):  # noqa: F811
+    """A cached length below zero is none, as step maps and attention take it; one near the largest number leaves room for the nodes, as step maps have it."""
+    n, most = 6, 6
+    chain, tables, lengths = [-1] + list(range(n - 1)), [[3, 1]] * 3, ints([-7] * 3)
+    got = accept(ops, [4] * (3 * n), [4] * (3 * n), chain * 3, [0, n, 2 * n, 3 * n], [-3, 2, 2 ** 31 - 1], tables, 4, 9, most, lengths)
+    want = plain_tree.accept([4] * (3 * n), [4] * (3 * n), chain * 3, [0, n, 2 * n, 3 * n], [0, 2, 2 ** 31 - 1], tables, 4, 9, most)
+    assert got == list(want)
+    assert lengths.tolist() == [6, 8, 2 ** 31 - 1]      # (the last: room for six nodes, all kept)
