@@ -541,7 +541,8 @@ void tree_attention(const TreeAttentionArgs& a, hipStream_t stream);
 size_t tree_attention_workspace_floats(int tokens, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_new, int max_cached, int window, int dtype);
 // choices[t]: the token chosen at node t, ids[t]: its drafted token. From the first node of a sequence on, to the first child whose token was
 // chosen: kept [n_seqs] nodes, their rows path [n_seqs, max_new] (-1 behind them), the token chosen at the last one, the page rows of
-// the kept nodes' keys and values, slots [tokens] (-1: not kept), and lengths[rows[b]] = cached[b] + kept[b] (lengths may be null).
+// the kept nodes' keys and values, slots [tokens] (-1: not kept), and lengths[rows[b]] = cached[b] + kept[b] (lengths may be null; of several
+// sequences of one request the last counts, and the others' slots are -1).
 struct TreeAcceptArgs {
     const int *choices = nullptr, *ids = nullptr, *parents = nullptr, *cu_q = nullptr, *cached = nullptr, *block_tables = nullptr, *rows = nullptr;
     int n_seqs = 0, tokens = 0, page_size = 0, n_pages = 0, max_blocks = 0, max_new = 0, n_requests = 0;

@@ -178,25 +178,25 @@ __global__ void __launch_bounds__(TREE_THREADS) tree_accept_kernel(TreeAcceptPar
     place = place_s[tid];
     const int kept = __syncthreads_count(place >= 0);
     int* path = a.path + static_cast<size_t>(b) * a.max_new;
+    // Of several sequences of one request the last one's length stands, and its nodes alone go to the pages: two sequences' keys in one row would be
+    // those that arrive last.
+    const int request = a.lengths == nullptr ? -1 : a.rows != nullptr ? a.rows[b] : b;
+    const bool named = static_cast<unsigned>(request) < static_cast<unsigned>(a.n_requests);
+    int later = 0;
+    if (named && a.rows != nullptr)
+        for (int i = b + 1 + tid; i < a.n_seqs; i += threads) later |= a.rows[i] == request;
+    later = __syncthreads_or(later);
     if (tid < n) {
-        a.slots[first + tid] = place >= 0 ? page_row(a.block_tables + static_cast<size_t>(b) * a.max_blocks, a.max_blocks, a.page_size, a.n_pages, cached + place) : -1;
+        a.slots[first + tid] = place >= 0 && !later ? page_row(a.block_tables + static_cast<size_t>(b) * a.max_blocks, a.max_blocks, a.page_size, a.n_pages, cached + place) : -1;
         if (place >= 0) path[place] = first + tid;
         if (place == kept - 1) a.next[b] = choice_s[tid];
     }
-    // (of several sequences of one request the last one's length stands)
-    int later = 0;
-    if (a.lengths != nullptr && a.rows != nullptr)
-        for (int i = b + 1 + tid; i < a.n_seqs; i += threads) later |= a.rows[i] == a.rows[b];
-    later = __syncthreads_or(later);
     for (int i = kept + tid; i < a.max_new; i += threads) path[i] = -1;
     for (int i = n + tid; i < all; i += threads) a.slots[first + i] = -1;
     if (tid == 0) {
         a.kept[b] = kept;
         if (kept == 0) a.next[b] = -1;
-        if (a.lengths != nullptr && !later) {
-            const int r = a.rows != nullptr ? a.rows[b] : b;
-            if (static_cast<unsigned>(r) < static_cast<unsigned>(a.n_requests)) a.lengths[r] = cached + kept;
-        }
+        if (named && !later) a.lengths[request] = cached + kept;
     }
 }
 

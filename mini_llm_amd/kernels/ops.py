@@ -906,8 +906,8 @@ def tree_accept(choices: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor,
     of its children whose token was chosen at it does. Writes, all int32: kept [n_seqs], the number of nodes that stand; path [n_seqs, max_new],
     their rows, -1 behind them; next_token [n_seqs], the choice at the last (a sequence without nodes: 0, -1, -1); slots [T], the page row of
     each node that stands (position cached[b] + its place on the path), -1 for the others and the rows of no sequence: what ``kv_append`` takes.
-    With ``lengths`` (int32 [requests]): lengths[rows[b]] = cached[b] + kept[b] (``rows`` None: b; of sequences of one request the last counts). Outputs lie
-    apart from the inputs and each other. A page that is none of the ``n_pages`` gives slot -1."""
+    With ``lengths`` (int32 [requests]): lengths[rows[b]] = cached[b] + kept[b] (``rows`` None: b; of sequences of one request the last counts, and
+    the others' nodes have slot -1). Outputs lie apart from the inputs and each other. A page that is none of the ``n_pages`` gives slot -1."""
     T, B = choices.numel(), cached.numel()
     tokens = [_counted(t, n, T) for t, n in ((choices, "choices"), (ids, "ids"), (parents, "parents"), (slots, "slots"))]
     at_cached, at_kept, at_next, at_cu = _counted(cached, "cached", B), _counted(kept, "kept", B), _counted(next_token, "next_token", B), _counted(cu_q, "cu_q", B + 1)

@@ -1,5 +1,5 @@
 """Drafted trees at the edges of what a call allows: maps used for trees and portions in turn, values and scores that are not finite or next to it, positions and
-lengths below zero; against the plain implementations in 64 bits (tests/plain_tree.py)."""
+lengths below zero, one request in several sequences; against the plain implementations in 64 bits (tests/plain_tree.py)."""
 import math
 import random
 
@@ -152,3 +152,21 @@ def test_tree_accept_takes_lengths_that_are_none_as_none(ops):  # noqa: F811
     want = plain_tree.accept([4] * (3 * n), [4] * (3 * n), chain * 3, [0, n, 2 * n, 3 * n], [0, 2, 2 ** 31 - 1], tables, 4, 9, most)
     assert got == list(want)
     assert lengths.tolist() == [6, 8, 2 ** 31 - 1]      # (the last: room for six nodes, all kept)
+
+
+def test_tree_accept_of_one_request_in_several_sequences_gives_page_rows_to_the_last(ops):  # noqa: F811
+    """Two sequences' keys in one row of the pages would be those that arrive last: the sequence whose length counts has them, the others' nodes go nowhere."""
+    B, n, R = 130, 3, 7
+    rng = random.Random(1)
+    rows = [rng.randrange(-1, R + 1) for _ in range(B)]
+    cached, tables = [rng.randint(0, 40) for _ in range(B)], [[rng.randrange(20) for _ in range(4)] for _ in range(B)]
+    choices, ids, parents, cu_q = [4] * (B * n), [rng.choice([4, 5]) for _ in range(B * n)], [-1, 0, 1] * B, list(range(0, B * n + 1, n))
+    lengths = ints([-7] * R)
+    got = accept(ops, choices, ids, parents, cu_q, cached, tables, 16, 20, n, lengths, rows)
+    want = list(plain_tree.accept(choices, ids, parents, cu_q, cached, tables, 16, 20, n))
+    last = {r: b for b, r in enumerate(rows)}
+    for b, r in enumerate(rows):
+        if 0 <= r < R and last[r] != b:
+            want[3][b * n:(b + 1) * n] = [-1] * n
+    assert got == want
+    assert lengths.tolist() == [cached[last[r]] + want[0][last[r]] if r in last else -7 for r in range(R)]
