@@ -150,6 +150,8 @@ __global__ void __launch_bounds__(TREE_THREADS) tree_accept_kernel(TreeAcceptPar
     const int first = min(max(a.cu_q[b], 0), a.tokens);
     if (b == a.n_seqs) {
         for (int t = first + tid; t < a.tokens; t += threads) a.slots[t] = -1;
+        const int ahead = min(max(a.cu_q[0], 0), a.tokens);          // (rows in front of the first sequence, where there are any)
+        for (int t = tid; t < ahead; t += threads) a.slots[t] = -1;
         return;
     }
     const int all = min(max(a.cu_q[b + 1] - first, 0), a.tokens - first), n = min(all, a.max_new);

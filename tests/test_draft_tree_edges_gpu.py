@@ -170,3 +170,15 @@ def test_tree_accept_of_one_request_in_several_sequences_gives_page_rows_to_the_
             want[3][b * n:(b + 1) * n] = [-1] * n
     assert got == want
     assert lengths.tolist() == [cached[last[r]] + want[0][last[r]] if r in last else -7 for r in range(R)]
+
+
+def test_tree_accept_of_rows_in_front_of_the_first_sequence(ops):  # noqa: F811
+    """Rows of no sequence go nowhere, in front of the first sequence as behind the last."""
+    T, cu_q = 300, [170, 172, 175]
+    parents, tables, lengths = [-1] * T, [[1, 2], [3, 4]], ints([0, 0])
+    for b in (0, 1):
+        for i in range(1, cu_q[b + 1] - cu_q[b]):
+            parents[cu_q[b] + i] = i - 1
+    args = [4] * T, [4] * T, parents, cu_q, [3, 5], tables, 4, 9, 3
+    assert accept(ops, *args, lengths) == list(plain_tree.accept(*args))
+    assert lengths.tolist() == [5, 8]
