@@ -4,13 +4,14 @@
 // The columns behind them are handed on as they are.
 //
 // The angle. f_i comes as a share of a turn per position in 64 bits of fixed point, so that position * f_i modulo 2^64 is the share of
-// a turn that is left, without any reduction: exact to position * 2^-65 turns at any 32-bit position, where a product of floats is off by
-// whole turns beyond 2^24. The quarter of a turn next to it is taken off in whole numbers; what is left, at most an eighth of a turn, goes to
+// a turn that is left, without any reduction and without an error of its own, where a product of floats is off by whole turns beyond 2^24. (The table's own
+// error counts position times: shares made in 64-bit floating point, as the framework's are, are off by up to 2^-54 turns.) The top 32 bits are taken. The quarter of a turn next to it is taken off in whole numbers; what is left, at most an eighth of a turn, goes to
 // a float (off by 2^-24 of itself) and into the series of sine and cosine, cut where the next term is below 2e-9 and 2e-10 of 1.
 //
 // Bound by memory: every row is read and written once. A thread has one place of a head (16 bytes; with halves the 16 bytes of both
 // halves), works out its angles once and goes through the heads with them. 8,192 rows of 40 heads of 128 in bfloat16 take 36 us, 4.6 TB/s, where a
-// copy of as many bytes reaches 5.2 (32 us); four heads' loads on their way at once instead of one's: 35.8 us, no more than runs differ. 200 rows of 18
+// copy of as many bytes reaches 5.2 (32 us); four heads' loads on their way at once instead of one's: 35.8 us, no more than runs differ. Where pairs, head or
+// strides do not fill 16 bytes it is a column (halves) or a pair (neighbours) at a time: 8,192 rows of 40 heads of 80 with 20 columns as halves take 79 us, 1.3 TB/s. 200 rows of 18
 // heads of 96 in 32 bits take 3.2 us, a launch; the call 7.1, which the host takes to make it.
 #include "common.h"
 

@@ -4,12 +4,13 @@
 // seen. With z_j = scale q_t . k_j over what is seen:
 //   o_t = sum_j exp(z_j - max z) v_j / sum_j exp(z_j - max z),   a node that sees nothing gets zeros.
 // What is not seen counts for nothing whatever stands there (infinities and NaN among it), and a block table's entry that names no page of
-// the pool holds nothing that is seen.
+// the pool holds nothing that is seen. What is seen counts as in the formula: a value that is not finite makes its column so in the rows that see it (NaN, where
+// its weight is zero in 32 bits), and a row all of whose seen keys score -inf is NaN.
 //
 // All nodes of a sequence and all query heads of a key/value head read the same keys, so these are the rows of one product (row r is node r /
-// group, head r % group of the key head's), of which a workgroup has up to 256. Keys and values come through LDS in stages, loaded straight
-// into it several stages ahead, so that what is on its way holds no register: a compute unit has up to 128 KB on its way where registers
-// would hold half of that. A workgroup's wavefronts are row groups x key groups: each has 16 RT rows, and of every stage the keys of its key
+// group, head r % group of the key head's), of which a workgroup has up to 256. Keys and values come through LDS in four stages of 32 KB, loaded straight
+// into it three stages ahead, so that what is on its way holds no register: 96 KB behind a request, of which 64 are still on their way when the next
+// stage is read. A workgroup's wavefronts are row groups x key groups: each has 16 RT rows, and of every stage the keys of its key
 // group; the key groups' states meet in LDS at the end. Few rows: one row group, many key groups, and memory is what bounds it; many rows: a
 // stage is read by all row groups, and the matrix instructions are.
 //
@@ -20,15 +21,16 @@
 //                 them, and takes the values of just these keys in 16 columns as the other operand. In bfloat16 these come out of LDS turned by
 //                 the read itself; in 32 bits a lane reads 16 (8) bytes at the same place c of a block of 256 (128) bytes: column m of the
 //                 product's tile x is column E m + x of the block, E words to a read.
-// Softmax statistics, sums and outputs are fp32; the weights are rounded to the values' type for the second product (in bfloat16: by half a step,
-// which averages over the keys; the sum is over the weights before they are rounded).
+// Softmax statistics, sums and outputs are fp32; the weights are rounded to the values' type for the second product. In bfloat16 that is half a step of each
+// (2^-8), which averages over the keys; the sum is over the rounded weights, as a product of ones with them, so that a row whose values are all alike gets that value. In 32 bits
+// nothing is rounded. (Weights kept in 32 bits would need the second product in 32 bits, at a sixteenth of the rate.)
 //
 // What bounds it, as measured in bfloat16 (a copy of 1 GiB reaches 5.2 TB/s, a product of 8,192 cubed 1.35 PFLOP/s):
 //   64 nodes over 31,000 positions, 25 heads of 64: 45 us, 4.5 TB/s: memory, and the join of 8 splits behind it (4 us).
-//   32 trees of up to 64 nodes over 4,096 to 8,192 positions, 32 query heads that share 8 of 128: 266 us, 0.59 PFLOP/s, 3.1 TB/s: what a unit has to do
-//   for a tile, at the clock that its power leaves. Matrix instructions are 45% of its cycles, softmax and addresses 35%; without loads from memory it takes 4% less; with the
-//   longest sequences' ends shared out to units that are done it takes as long.
-//   8 sequences of one node over 1,000 positions, 12 heads of 64: 12 us, of which 8 are a launch, three loads that wait for each other (lengths, table,
+//   32 trees of up to 64 nodes over 4,096 to 8,192 positions, 32 query heads that share 8 of 128: 262 to 276 us by the machine, 0.59 PFLOP/s, 3.1 TB/s: what a unit has
+//   to do for a tile, and units that are done: they are busy in 73% of the kernel's cycles (at 2.38 GHz), of which matrix instructions take 45%, softmax and addresses 34%; without
+//   loads from memory it takes 4% less; with the longest sequences' ends shared out to units that are done it took as long.
+//   8 sequences of one node over 1,000 positions, 12 heads of 64: 12.2 us, of which 8 are a launch, three loads that wait for each other (lengths, table,
 //   keys) and the merge.
 // What the steps to this gave (us; these three calls, and one of 3 trees of 37 nodes with a window of 1,000, 10 heads of 80 that share 5): a workgroup a
 // row and head, keys straight from memory: 17,689, 101,655, 501, 732; on the matrix cores with LDS stages: 51, 313, 15, 27; the way of sharing
@@ -827,8 +829,7 @@ constexpr Way NARROW[] = {{1, 4, 4}, {1, 8, 4}, {1, 8, 2}, {2, 8, 2}, {2, 8, 1}}
 // Of every way and number of splits the one whose time is the least by a sum of what was measured, in us: a step (a wavefront's keys of a
 // stage) takes 0.8 and its products, workgroups beyond the compute units take turns, all stages together come at 4.2 TB/s, and a
 // join takes 6 and 0.2 a split (2.5 of it on the unit's side, the rest the host's: a second launch and a workspace, 14 us a call instead of 11). Over 180 calls
-// in all ways of sharing them out the times taken, the host's among them, lie 3% above the best on average (61% at most); with a join at 2.5 4%, with
-// fixed bounds on rows and keys, over the first 64 of them, 21%.
+// in all ways of sharing them out the times taken, the host's among them, lie 4% above the best on average (58% at most), and 6% by the GPU's alone.
 Plan plan_of(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_new, int max_cached, int window, int dtype) {
     const bool f32 = dtype == MLLM_F32;
     const int nt = head_dim <= 32 ? 1 : head_dim <= 64 ? 2 : head_dim <= 128 ? 4 : 8, keys = f32 ? 16 : 32;
@@ -919,7 +920,7 @@ int mllm_tree_attention(const void* q, long long ldq, const void* k, long long l
     p.page_shift = 31 + bits;
     p.page_magic = static_cast<unsigned>(((1ull << p.page_shift) + page_size - 1) / page_size);
     p.row_tiles = plan.row_tiles; p.nsplit = plan.nsplit; p.units = static_cast<int>(units);
-    // (a scale of zero: so small that every finite product becomes zero by it, and -inf stays)
+    // (a scale of zero, or one next to it: so small that products up to 2^98 move no weight by more than half a step, and -inf stays)
     p.scale = std::max(std::fabs(scale) * MLLM_LOG2E, 1e-37f);
     p.negative = scale < 0.f;
     p.out = static_cast<char*>(out); p.ws = ws;

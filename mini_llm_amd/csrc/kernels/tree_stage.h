@@ -42,7 +42,8 @@ struct Stage {
     static constexpr int KEYS = keys();
     static constexpr int TURNS = KEYS / LEAST;                            // tiles of a key group in a stage
     static constexpr int MATRIX = KEYS * ROW, BYTES = 2 * MATRIX;
-    static constexpr int NUMBER = 4 * BYTES <= 131072 ? 4 : 3;            // one is read, the next has come, the others are on their way
+    static constexpr int NUMBER = 4;          // of stages in LDS: one is read, the next has come, the others are on their way
+    static_assert(NUMBER * BYTES <= 131072, "beside the table and the states");
     static constexpr int LOADS = KEYS * PIECES / 64 / NW;                 // of a wavefront, a stage and matrix
     static_assert(LOADS * 64 * NW == KEYS * PIECES, "whole instructions");
     static constexpr int MINE = KEYS / NW, PER_LOAD = 64 / PIECES;        // rows of a wavefront (it loads these), rows of a load instruction

@@ -767,7 +767,7 @@ def step_maps(maps: StepMaps, rows: Optional[torch.Tensor], n_new: torch.Tensor,
     ancestors those of a chain). With ``parents`` (int32
     [tokens], needs maps made with ``tree=True``) they are a tree each: positions are lengths[r] + depth, slots -1 (``tree_accept``
     says later where the kept ones go), ancestors the sets that ``tree_attention`` takes; a parent that does not stand in front of its
-    child counts as none. The maps' arrays lie apart from the inputs. More than ``max_new`` tokens of a sequence, or more than ``tokens`` together, are left out (cu_q says how
+    child counts as none. Several trees may be one request's; portions of one request in two sequences would have the same page rows. The maps' arrays lie apart from the inputs. More than ``max_new`` tokens of a sequence, or more than ``tokens`` together, are left out (cu_q says how
     many are in). A position beyond ``max_blocks``, or whose page is none of the ``n_pages``, has slot -1. Tokens behind the last sequence get
     sequence 0, position 0, slot -1 and no ancestors."""
     B, T, blocks, mine = maps.n_seqs, maps.tokens, maps.max_blocks, maps.addresses
@@ -801,7 +801,10 @@ def rotary_freqs(rot_dims: int, base: float = 10000.0, scaling: Optional[dict] =
       fastest not at all;
     * ``{"kind": "by_turns", "factor": s, "original": n, "fast": f, "slow": w}``: f_i where the pair makes at least f turns over the n
       positions of training, f_i / s where it makes at most w, between them the mixture that is linear in its turns;
-    * ``{"kind": "by_pair", ...}`` (the same numbers): the mixture linear in the pair's number, between the (fractional) pairs that make f and w turns."""
+    * ``{"kind": "by_pair", ...}`` (the same numbers): the mixture linear in the pair's number, between the (fractional) pairs that make f and w turns.
+
+    The shares are worked out in 64-bit floating point and off by up to 2^-54 of a turn, which an angle has as many times as its position says: less than 2^-32 of
+    a turn up to position 2^22, about 2^-23 at the ends of 32 bits."""
     if rot_dims < 2 or rot_dims % 2 or not base > 0.0 or not math.isfinite(base):
         raise KernelError(f"rotary positions of {rot_dims} columns with base {base}: columns come in pairs, the base is positive")
     kind = None if scaling is None else scaling.get("kind")
@@ -840,8 +843,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, n_head
            amplitude: float = 1.0) -> torch.Tensor:
     """out = x [T, n_heads * head_dim] (float32 or bfloat16, any row stride) with pair i < len(freqs) of every head turned by the angle
     positions[t] * freqs[i] (``rotary_freqs``) and multiplied by ``amplitude``; pairs are columns i and i + len(freqs) of a head, or 2i and
-    2i + 1 with ``interleaved``; the columns behind them are handed on. ``out`` may be ``x``. positions: int32 [T], in any order; angles
-    are exact to 2^-32 of a turn at any of them."""
+    2i + 1 with ``interleaved``; the columns behind them are handed on. ``out`` may be ``x``. positions: int32 [T], in any order; the
+    angle is that product to 2^-32 of a turn at any of them (what the frequencies themselves are off by, ``rotary_freqs``, counts as often as the position says)."""
     if freqs.dim() != 1 or freqs.dtype is not torch.int64 or not freqs.is_contiguous() or freqs.numel() < 1:
         raise KernelError("freqs must be contiguous int64 [pairs] (rotary_freqs)")
     if x.dim() != 2 or x.shape != out.shape:
