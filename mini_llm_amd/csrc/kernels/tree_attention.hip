@@ -750,8 +750,7 @@ __global__ void __launch_bounds__(NW * 64) tree_attention_kernel(TreeAttentionPa
             const float2 ml = ml_s[at + i * 16 * RT];
             const f32x4 part = *reinterpret_cast<const f32x4*>(state_s + (at + i * 16 * RT) * PITCH + d);
             const float weight = exp2_for<T>(ml.x - top);
-            if (ml.y == 0.f) continue;          // (a key group whose keys nobody saw)
-            sum += weight * ml.y;
+            sum += weight * ml.y;               // (a key group whose keys nobody saw has zeros)
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] += weight * part[e];
         }
@@ -801,7 +800,7 @@ __global__ void __launch_bounds__(256) tree_attention_join_kernel(TreeAttentionP
             for (int j = 0; j < 4; ++j) v[j] *= kept;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const bool counts = s0 + i <= last && ml[i].y != 0.f;
+                const bool counts = s0 + i <= last;
                 const float weight = exp2_for<T>(ml[i].x - top);
                 sum += counts ? weight * ml[i].y : 0.f;
 #pragma unroll

@@ -182,3 +182,17 @@ def test_tree_accept_of_rows_in_front_of_the_first_sequence(ops):  # noqa: F811
     args = [4] * T, [4] * T, parents, cu_q, [3, 5], tables, 4, 9, 3
     assert accept(ops, *args, lengths) == list(plain_tree.accept(*args))
     assert lengths.tolist() == [5, 8]
+
+
+@pytest.mark.parametrize("dtype,seqs,Hkv,group,most,dim,hint", WAYS)
+def test_tree_attention_of_an_infinite_value_whose_key_scores_minus_infinity(ops, dtype, seqs, Hkv, group, most, dim, hint):  # noqa: F811
+    """Zero times infinity too where all keys that a part of the call looks at score so: every key but the nodes' and the first of the cache."""
+    c = way_case(dtype, seqs, Hkv, group, most, dim)
+    for b in range(seqs):
+        for at in range(1, c.cached[b]):
+            c.k_pages[c.tables[b][at // c.page] * c.page + at % c.page, 0::dim] = -math.inf
+        if c.cached[b] > 1 and b % 2 == 0:
+            at = 1 + (7 * b + 40) % (c.cached[b] - 1)
+            c.v_pages[c.tables[b][at // c.page] * c.page + at % c.page, 1::dim] = math.inf
+    want = same_with_what_is_not_finite(c, c.call(ops, c.device(), max_cached=hint))
+    assert torch.isfinite(want[:, 0]).all()
