@@ -28,9 +28,9 @@
 // What bounds it, as measured in bfloat16 (a copy of 1 GiB reaches 5.2 TB/s, a product of 8,192 cubed 1.35 PFLOP/s):
 //   64 nodes over 31,000 positions, 25 heads of 64: 45 us, 4.5 TB/s: memory, and the join of 8 splits behind it (4 us).
 //   32 trees of up to 64 nodes over 4,096 to 8,192 positions, 32 query heads that share 8 of 128: 262 to 276 us by the machine, 0.59 PFLOP/s, 3.1 TB/s: what a unit has
-//   to do for a tile, and units that are done: they are busy in 73% of the kernel's cycles (at 2.38 GHz), of which matrix instructions take 45%, softmax and addresses 34%; without
+//   to do for a tile, and units that are done: they are busy in 73% of the kernel's cycles (at 2.4 GHz), of which matrix instructions take 44%, softmax and addresses 34%; without
 //   loads from memory it takes 4% less; with the longest sequences' ends shared out to units that are done it took as long.
-//   8 sequences of one node over 1,000 positions, 12 heads of 64: 12.2 us, of which 8 are a launch, three loads that wait for each other (lengths, table,
+//   8 sequences of one node over 1,000 positions, 12 heads of 64: 11.9 us, of which 8 are a launch, three loads that wait for each other (lengths, table,
 //   keys) and the merge.
 // What the steps to this gave (us; these three calls, and one of 3 trees of 37 nodes with a window of 1,000, 10 heads of 80 that share 5): a workgroup a
 // row and head, keys straight from memory: 17,689, 101,655, 501, 732; on the matrix cores with LDS stages: 51, 313, 15, 27; the way of sharing
@@ -828,7 +828,7 @@ constexpr Way NARROW[] = {{1, 4, 4}, {1, 8, 4}, {1, 8, 2}, {2, 8, 2}, {2, 8, 1}}
 // Of every way and number of splits the one whose time is the least by a sum of what was measured, in us: a step (a wavefront's keys of a
 // stage) takes 0.8 and its products, workgroups beyond the compute units take turns, all stages together come at 4.2 TB/s, and a
 // join takes 6 and 0.2 a split (2.5 of it on the unit's side, the rest the host's: a second launch and a workspace, 14 us a call instead of 11). Over 180 calls
-// in all ways of sharing them out the times taken, the host's among them, lie 4% above the best on average (58% at most), and 6% by the GPU's alone.
+// in all ways of sharing them out the times taken, the host's among them, lie 4.5% above the best on average (58% at most), and 5% by the GPU's alone.
 Plan plan_of(int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_new, int max_cached, int window, int dtype) {
     const bool f32 = dtype == MLLM_F32;
     const int nt = head_dim <= 32 ? 1 : head_dim <= 64 ? 2 : head_dim <= 128 ? 4 : 8, keys = f32 ? 16 : 32;

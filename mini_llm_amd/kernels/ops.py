@@ -869,7 +869,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, n_heads: i
     projection's rows), head_dim a multiple of 8 up to 256, out like q, apart from the inputs. block_tables: int32 [n_seqs, max_blocks], cached [n_seqs], cu_q
     [n_seqs + 1], ancestors int64 [T, words], positions [T] (only with a window). No sequence brings more than ``max_new`` <= 64 * words nodes
     (those beyond are not computed); ``max_cached``, the longest cache, decides how the keys are shared out. A node that sees nothing gets zeros;
-    rows of no sequence stay as they are; what is not seen counts for nothing, NaN among it; a table's entry that names no page holds nothing."""
+    rows of no sequence stay as they are; what is not seen counts for nothing, NaN among it, and what is seen counts as in the formula (NaN where all that is seen
+    scores -inf, or where an infinite value's weight is zero in 32 bits); a table's entry that names no page holds nothing."""
     T, B = q.shape[0], cached.numel()
     at_tables, blocks = _whole_table(block_tables, "block_tables", B)
     at_cached, at_cu, at_positions = _counted(cached, "cached", B), _counted(cu_q, "cu_q", B + 1), 0
